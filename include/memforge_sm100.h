@@ -367,6 +367,126 @@ typedef struct {
 MF_API int mf_accept_commit(const mf_accept_args* args, mf_stream_t stream);
 
 /*
+ * Score modifiers of an attention call (no counterpart in the reference; models
+ * ask for them through the attention function's softcap / sliding_window).  For
+ * the row at position p and key position k, in this order:
+ *   s = scale * q.k
+ *   softcap > 0:       s = softcap * tanh(s / softcap)
+ *   alibi_slopes:      s = s - alibi_slopes[query head] * (p - k)
+ *   visible iff        k < kv_len and (k < prefix_lens[seq] or
+ *                      ((not causal or k <= p) and (window == 0 or p - k < window)))
+ * where row i of a sequence is at p = kv_len - q_len + i.  A prefix is seen by every
+ * row, earlier ones included, and stays visible behind a window.  A row that sees no key is
+ * written as zeros.  A zero / NULL member leaves its step out; softcap and window
+ * must not be negative.
+ */
+typedef struct {
+  float softcap;
+  int32_t window;
+  const float* alibi_slopes;  /* [num_q_heads] or NULL */
+  const int32_t* prefix_lens; /* [num_seqs] or NULL */
+} mf_score_mods;
+
+/*
+ * mf_paged_attention with modified scores, over a 16- or 32-bit pool.  Arguments
+ * as there; `mods` must not be NULL.  A side window (win_k) and peer output are
+ * not served with modifiers (MF_EUNSUPPORTED).  The workspace rules are those of
+ * mf_paged_attention.
+ */
+MF_API size_t mf_paged_attention_scored_workspace_size(const mf_attention_args* args,
+                                                       const mf_score_mods* mods, int device);
+MF_API int mf_paged_attention_scored(const mf_attention_args* args, const mf_score_mods* mods,
+                                     void* workspace, size_t workspace_bytes,
+                                     int32_t* err_flag, mf_stream_t stream);
+
+/*
+ * The 4-bit KV cache (no counterpart in the reference).  One layer's pool holds,
+ * for each (block of 16 tokens, kv head), one record of mf_q4_record_bytes(D) =
+ * 16 * D + 128 contiguous bytes at pool + block * stride_block + head * stride_head
+ * (strides in bytes, multiples of 16; D is 64, 128 or 256).  A row x of D values (one
+ * token, kv head, K or V) is held as 4-bit codes n and two fp16 numbers:
+ *   base  = the largest fp16 not above min(x)
+ *   scale = the smallest fp16 with 15 * scale >= max(x) - base
+ *   n     = (x - base) / scale, rounded to nearest even;   x is read as n * scale + base
+ * A row with a NaN or a magnitude above 65504 has NaN for both and reads as NaN.
+ * Record:
+ *   [0, 8D)        K codes: token t at t * D/2, the even dim in a byte's low nibble
+ *   [8D, 16D)      V codes: [C][t >> 3][8][(t >> 1) & 3][W][t & 1][2 bytes] with
+ *                  C = max(1, D / 128), W = min(4, D / 32); chunk c, group g, word w
+ *                  hold dims 128 c + 4W g + 4w .. + 3, even dims in the low nibbles
+ *   [16D, +64)     K parameters: (scale, base) of each token
+ *   [16D + 64, +64) V parameters
+ */
+MF_API int64_t mf_q4_record_bytes(int32_t head_dim); /* negative: unsupported head_dim */
+
+/*
+ * Quantising form of mf_reshape_and_cache: token t, head h of key / value goes to
+ * slot slot_mapping[t] (-1 skips the token; a slot outside the pool sets MF_ERR_SLOT).
+ * Sources are fp32, fp16 or bf16.  Two tokens naming one slot race.
+ */
+MF_API int mf_q4_reshape_and_cache(const void* key, const void* value, mf_dtype src_dtype,
+                                   int64_t k_stride_tok, int64_t k_stride_head,
+                                   int64_t v_stride_tok, int64_t v_stride_head, void* pool,
+                                   int64_t pool_stride_block, int64_t pool_stride_head,
+                                   int32_t num_blocks, const void* slot_mapping,
+                                   int32_t slot_mapping_is_int64, int32_t num_tokens,
+                                   int32_t num_kv_heads, int32_t head_dim, int32_t* err_flag,
+                                   mf_stream_t stream);
+
+/*
+ * Dequantising form of mf_gather_kv: n * scale + base in fp32 (one fused
+ * multiply-add), rounded to out_dtype.  An index outside the pool sets MF_ERR_SLOT
+ * and yields zeros.
+ */
+MF_API int mf_q4_gather_kv(const void* pool, int64_t pool_stride_block, int64_t pool_stride_head,
+                           int32_t num_blocks, const void* flat_index, int32_t index_is_int64,
+                           int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                           void* key_out, void* value_out, mf_dtype out_dtype,
+                           int64_t out_stride_head, int64_t out_stride_tok, int32_t* err_flag,
+                           mf_stream_t stream);
+
+/*
+ * Attention over a 4-bit pool: rows, tables, lengths and masks as in
+ * mf_paged_attention (q_per_seq or cu_seqlens_q; decode, verify and chunks), q and
+ * out of `dtype`, with the score modifiers of `mods` (all zero: none).  Every row of
+ * the run is read from the pool: write the step's keys first.  A row without a
+ * visible key (kv_len 0, or kv_len < q_len) is written as zeros, without an error.
+ * A negative kv_len or a run longer than max_q_len sets MF_ERR_LENGTH, a table too short
+ * for kv_len MF_ERR_TABLE (the keys behind it are left out), a block id outside the
+ * pool MF_ERR_BLOCK_ID (block 0 is read in its place).
+ *
+ * The workspace (16-byte aligned) is scratch: it needs no initial value and nothing
+ * in it outlives the call, but calls that may overlap must not share one.
+ */
+typedef struct {
+  uint32_t struct_size; /* sizeof(mf_q4_attention_args) */
+  const void* q;        /* [rows][num_q_heads][head_dim] */
+  int64_t q_stride_row, q_stride_head;
+  void* out;
+  int64_t out_stride_row, out_stride_head;
+  const void* pool; /* one layer */
+  int64_t pool_stride_block, pool_stride_head; /* bytes */
+  int32_t num_blocks;
+  const int32_t* block_tables; /* [num_seqs], rows table_stride entries apart */
+  int32_t table_stride;
+  int32_t table_width;         /* entries of a row */
+  const int32_t* cu_seqlens_q; /* [num_seqs + 1] or NULL */
+  int32_t q_per_seq;           /* used when cu_seqlens_q is NULL */
+  const int32_t* kv_lens;      /* [num_seqs] */
+  const int32_t* row_map;      /* [total_q] or NULL */
+  int32_t num_seqs, total_q, max_q_len;
+  int32_t num_q_heads, num_kv_heads, head_dim;
+  float scale;
+  int32_t causal;
+  mf_dtype dtype;
+  mf_score_mods mods;
+} mf_q4_attention_args;
+
+MF_API size_t mf_q4_paged_attention_workspace_size(const mf_q4_attention_args* args, int device);
+MF_API int mf_q4_paged_attention(const mf_q4_attention_args* args, void* workspace,
+                                 size_t workspace_bytes, int32_t* err_flag, mf_stream_t stream);
+
+/*
  * Copy-on-write block copy across all layers: for each pair i, block
  * src[i] -> dst[i] in every layer of both pools (prefix_sharing.copy_block,
  * memforge_ml/runtime/prefix_sharing.py:28-42).  Pools are contiguous

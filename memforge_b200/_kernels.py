@@ -21,9 +21,11 @@ Workspace and error word
 
 from __future__ import annotations
 
+import ctypes
 import os
 import threading
-from typing import Dict, Optional, Sequence
+from contextlib import nullcontext
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
@@ -38,7 +40,8 @@ _err_words: Dict[int, torch.Tensor] = {}
 _checks = os.environ.get("MEMFORGE_CHECK", "0") not in ("", "0")
 launch_counter = {"reshape_and_cache": 0, "paged_attention": 0, "copy_blocks": 0,
                   "peer_barrier": 0, "commit_window": 0, "gather_kv": 0,
-                  "accept_commit": 0}
+                  "accept_commit": 0, "scored_attention": 0, "q4_reshape_and_cache": 0,
+                  "q4_gather_kv": 0, "q4_paged_attention": 0}
 
 
 def set_checks(enabled: bool) -> None:
@@ -117,6 +120,20 @@ def _after(what: str, device: torch.device) -> None:
     if _checks:
         torch.cuda.synchronize(device)
         check_device_errors(device)
+
+
+def _on(device: torch.device):
+    """The tensors' device as the current one for a launch."""
+    if device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
+
+
+def require_one_device(what: str, device: torch.device, *tensors) -> None:
+    require_cuda(what, *tensors)
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -303,8 +320,10 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, key_pool: torch.Tensor,
                     causal: bool = True, row_map: Optional[torch.Tensor] = None,
                     win_k: Optional[torch.Tensor] = None, win_v: Optional[torch.Tensor] = None,
                     heads_major: bool = False, workspace_tensor: Optional[torch.Tensor] = None,
-                    out_peers: Optional[Sequence[int]] = None, out_head_offset: int = 0
-                    ) -> torch.Tensor:
+                    out_peers: Optional[Sequence[int]] = None, out_head_offset: int = 0,
+                    softcap: float = 0.0, window: int = 0,
+                    alibi_slopes: Optional[torch.Tensor] = None,
+                    prefix_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
     """
     ``mf_paged_attention`` on torch tensors.
 
@@ -317,6 +336,10 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, key_pool: torch.Tensor,
     out_peers: device addresses of the full ``[rows, total heads, D]`` output on
     every GPU of a head-sharded step (``out`` gives their strides); the kernel
     stores this call's heads at ``out_head_offset`` into all of them.
+    softcap / window / alibi_slopes / prefix_lens: the score modifiers of
+    ``mf_paged_attention_scored`` (0 or None: none; slopes fp32 ``[Hq]``, prefixes int32
+    ``[num_seqs]``).  Without ``workspace_tensor`` a call with modifiers uses a
+    workspace of its device and stream, and inside a graph capture one of its own.
     """
     require_cuda("paged_attention", q, out, key_pool, value_pool, block_tables, kv_lens,
                  cu_seqlens_q, row_map, win_k, win_v)
@@ -373,6 +396,20 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, key_pool: torch.Tensor,
     lib = L.lib()
     dev = q.device
     idx = _dev_index(q)
+    mods = score_mods(dev, hq, num_seqs, softcap, window, alibi_slopes, prefix_lens)
+    if mods is not None:
+        require_one_device("paged_attention", dev, out, key_pool, value_pool, block_tables,
+                           kv_lens, cu_seqlens_q, row_map)
+        with _on(dev):
+            need = lib.mf_paged_attention_scored_workspace_size(a, mods, idx)
+            ws = workspace_tensor if workspace_tensor is not None else (
+                stream_workspace(dev, need) if need else None)
+            rc = lib.mf_paged_attention_scored(a, mods, _ptr(ws), 0 if ws is None else ws.numel(),
+                                               err_word(dev).data_ptr(), _stream_ptr(dev))
+        L.check(rc, "mf_paged_attention_scored")
+        launch_counter["scored_attention"] += 1
+        _after("scored_attention", dev)
+        return out
     need = lib.mf_paged_attention_workspace_size(a, idx)
     ws = workspace_tensor if workspace_tensor is not None else (
         workspace(dev, need) if need else None)
@@ -384,13 +421,220 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, key_pool: torch.Tensor,
     return out
 
 
+def score_mods(device: torch.device, num_q_heads: int, num_seqs: int, softcap: float, window: int,
+               alibi_slopes: Optional[torch.Tensor],
+               prefix_lens: Optional[torch.Tensor]) -> Optional[L.ScoreMods]:
+    """The checked ``mf_score_mods``, or None when no modifier is given."""
+    if not softcap and not window and alibi_slopes is None and prefix_lens is None:
+        return None
+    if not 0.0 <= softcap <= 1e30:
+        raise ValueError(f"softcap must be 0 (none) or positive, got {softcap}")
+    if window < 0:
+        raise ValueError(f"window must be 0 (none) or positive, got {window}")
+    for name, t, dt, n in (("alibi_slopes", alibi_slopes, torch.float32, num_q_heads),
+                           ("prefix_lens", prefix_lens, torch.int32, num_seqs)):
+        if t is None:
+            continue
+        if t.device != device or t.dtype != dt or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be {n} contiguous {dt} values on {device}, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return L.ScoreMods(float(softcap), int(window), _ptr(alibi_slopes), _ptr(prefix_lens))
+
+
+_stream_workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
+
+
+def stream_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """
+    A zeroed-counter workspace that no other stream uses: one per (device, stream), or,
+    inside a graph capture, memory of that graph whose counters the graph clears.
+    """
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:min(nbytes, 1 << 20)].zero_()   # the arrival counters at its front
+        return ws
+    key = (device.index, _stream_ptr(device))
+    ws = _stream_workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        _stream_workspaces[key] = ws
+    return ws
+
+
+# ------------------------------------------------------------- 4-bit KV cache
+
+Q4_BLOCK = 16
+
+
+def q4_head_dim(pool: torch.Tensor) -> int:
+    """head_dim of a 4-bit pool layer ``(blocks, kv_heads, 16 * D + 128)``, checked."""
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.stride(-1) != 1:
+        raise ValueError(f"a 4-bit pool layer is uint8 (blocks, kv_heads, 16 * D + 128) with "
+                         f"contiguous records, got {pool.dtype} {tuple(pool.shape)}")
+    d = (pool.shape[2] - 128) // 16
+    if d not in (64, 128, 256) or pool.shape[2] != 16 * d + 128:
+        raise ValueError(f"no head_dim of 64, 128 or 256 has records of {pool.shape[2]} bytes")
+    return d
+
+
+def _slots(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be int32 or int64")
+    return t.reshape(-1).contiguous()
+
+
+def q4_reshape_and_cache(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor,
+                         slot_mapping: torch.Tensor) -> None:
+    """
+    ``mf_q4_reshape_and_cache``: quantise ``key``/``value`` rows ``(T, H, D)`` (fp32,
+    fp16 or bf16, any token and head strides) into one 4-bit pool layer
+    ``(blocks, H, 16 * D + 128)`` at ``slot_mapping[t]`` (-1 = skip).
+    """
+    dev = pool.device
+    require_one_device("q4_reshape_and_cache", dev, pool, key, value, slot_mapping)
+    D = q4_head_dim(pool)
+    if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError(f"keys/values must be (T, H, D) of one shape and dtype, got "
+                         f"{tuple(key.shape)} {key.dtype} and {tuple(value.shape)} {value.dtype}")
+    T, H, d = key.shape
+    if (H, d) != (pool.shape[1], D):
+        raise ValueError(f"pool holds {pool.shape[1]} heads x {D} dims, keys are {H} x {d}")
+    if key.stride(-1) != 1:
+        key = key.contiguous()
+    if value.stride(-1) != 1:
+        value = value.contiguous()
+    slots = _slots("slot_mapping", slot_mapping)
+    if slots.numel() != T:
+        raise ValueError(f"{T} tokens but {slots.numel()} slots")
+    code = dtype_code(key.dtype)
+    if T == 0:
+        return
+    with _on(dev):
+        rc = L.lib().mf_q4_reshape_and_cache(
+            key.data_ptr(), value.data_ptr(), code, key.stride(0), key.stride(1), value.stride(0),
+            value.stride(1), pool.data_ptr(), pool.stride(0), pool.stride(1), pool.shape[0],
+            slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, T, H, D,
+            err_word(dev).data_ptr(), _stream_ptr(dev))
+    L.check(rc, "mf_q4_reshape_and_cache")
+    launch_counter["q4_reshape_and_cache"] += 1
+    _after("q4_reshape_and_cache", dev)
+
+
+def q4_gather_kv(pool: torch.Tensor, flat_index: torch.Tensor,
+                 dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """
+    ``mf_q4_gather_kv``: slots ``flat_index`` of one 4-bit pool layer, dequantised to
+    contiguous ``(1, H, T, D)`` keys and values of ``dtype``.
+    """
+    dev = pool.device
+    require_cuda("q4_gather_kv", pool)
+    D = q4_head_dim(pool)
+    code = dtype_code(dtype)
+    if flat_index.device != dev:
+        flat_index = flat_index.to(dev)
+    index = _slots("flat_index", flat_index)
+    T, H = index.numel(), pool.shape[1]
+    k = torch.empty((1, H, T, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if T == 0:
+        return k, v
+    with _on(dev):
+        rc = L.lib().mf_q4_gather_kv(
+            pool.data_ptr(), pool.stride(0), pool.stride(1), pool.shape[0], index.data_ptr(),
+            1 if index.dtype == torch.int64 else 0, T, H, D, k.data_ptr(), v.data_ptr(), code,
+            T * D, D, err_word(dev).data_ptr(), _stream_ptr(dev))
+    L.check(rc, "mf_q4_gather_kv")
+    launch_counter["q4_gather_kv"] += 1
+    _after("q4_gather_kv", dev)
+    return k, v
+
+
+def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
+                       block_tables: torch.Tensor, kv_lens: torch.Tensor, *,
+                       cu_seqlens_q: Optional[torch.Tensor] = None, q_per_seq: int = 1,
+                       max_q_len: Optional[int] = None, scale: float, causal: bool = True,
+                       row_map: Optional[torch.Tensor] = None, softcap: float = 0.0,
+                       window: int = 0, alibi_slopes: Optional[torch.Tensor] = None,
+                       prefix_lens: Optional[torch.Tensor] = None,
+                       workspace_tensor: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """
+    ``mf_q4_paged_attention`` on torch tensors: q, out ``(rows, Hq, D)`` views (any row
+    and head strides, D contiguous), one 4-bit pool layer, and tables, lengths,
+    rows and score modifiers as in :func:`paged_attention`.  The workspace is scratch
+    of the caching allocator unless one is given.
+    """
+    dev = q.device
+    require_one_device("q4_paged_attention", dev, q, out, pool, block_tables, kv_lens,
+                       cu_seqlens_q, row_map, workspace_tensor)
+    D = q4_head_dim(pool)
+    for name, t in (("block_tables", block_tables), ("kv_lens", kv_lens),
+                    ("cu_seqlens_q", cu_seqlens_q), ("row_map", row_map)):
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32 (got {t.dtype})")
+    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"q and out must be (rows, heads, D) of one shape and dtype, got "
+                         f"{tuple(q.shape)} {q.dtype} and {tuple(out.shape)} {out.dtype}")
+    if q.stride(-1) != 1 or out.stride(-1) != 1:
+        raise ValueError("q/out need a contiguous head_dim")
+    rows, hq, d = q.shape
+    hkv = pool.shape[1]
+    if d != D:
+        raise ValueError(f"query head_dim {d} but the pool holds {D}")
+    if hq % hkv:
+        raise ValueError(f"{hq} query heads is not a multiple of {hkv} kv heads")
+    num_seqs = kv_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs:
+        raise ValueError("block_tables must be [num_seqs, width]")
+    if cu_seqlens_q is not None:
+        if cu_seqlens_q.numel() != num_seqs + 1 or max_q_len is None:
+            raise ValueError("cu_seqlens_q needs num_seqs + 1 offsets and max_q_len")
+        cu_seqlens_q = cu_seqlens_q.contiguous()
+    elif q_per_seq * num_seqs != rows:
+        raise ValueError(f"{num_seqs} sequences of {q_per_seq} rows but {rows} query rows")
+    if row_map is not None and (row_map.numel() != rows or not row_map.is_contiguous()):
+        raise ValueError("row_map must be contiguous with one entry per row")
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    kv_lens = kv_lens.contiguous()
+    a = L.Q4AttentionArgs()
+    a.struct_size = ctypes.sizeof(L.Q4AttentionArgs)
+    a.q, a.q_stride_row, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1)
+    a.out, a.out_stride_row, a.out_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
+    a.pool, a.pool_stride_block, a.pool_stride_head = (pool.data_ptr(), pool.stride(0),
+                                                       pool.stride(1))
+    a.num_blocks = pool.shape[0]
+    # A row of the table holds `width` entries; rows may lie further apart.
+    a.block_tables, a.table_stride = block_tables.data_ptr(), block_tables.stride(0)
+    a.table_width = block_tables.shape[1]
+    a.cu_seqlens_q, a.q_per_seq = _ptr(cu_seqlens_q), q_per_seq
+    a.kv_lens, a.row_map = kv_lens.data_ptr(), _ptr(row_map)
+    a.num_seqs, a.total_q = num_seqs, rows
+    a.max_q_len = max_q_len if max_q_len is not None else q_per_seq
+    a.num_q_heads, a.num_kv_heads, a.head_dim = hq, hkv, D
+    a.scale, a.causal, a.dtype = float(scale), 1 if causal else 0, dtype_code(q.dtype)
+    mods = score_mods(dev, hq, num_seqs, softcap, window, alibi_slopes, prefix_lens)
+    if mods is not None:
+        a.mods = mods
+    lib = L.lib()
+    with _on(dev):
+        need = lib.mf_q4_paged_attention_workspace_size(a, dev.index)
+        ws = workspace_tensor
+        if ws is None:
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        rc = lib.mf_q4_paged_attention(a, ws.data_ptr(), ws.numel() * ws.element_size(),
+                                       err_word(dev).data_ptr(), _stream_ptr(dev))
+    L.check(rc, "mf_q4_paged_attention")
+    launch_counter["q4_paged_attention"] += 1
+    _after("q4_paged_attention", dev)
+    return out
+
+
 _ARGS_SIZE = None
 
 
 def ctypes_sizeof_args() -> int:
     global _ARGS_SIZE
     if _ARGS_SIZE is None:
-        import ctypes
         _ARGS_SIZE = ctypes.sizeof(L.AttentionArgs)
     return _ARGS_SIZE
 
@@ -398,7 +642,6 @@ def ctypes_sizeof_args() -> int:
 def peer_barrier(flag_ptrs: Sequence[int], rank: int, epoch: int,
                  device: torch.device) -> None:
     """``mf_peer_barrier``: completes a head-sharded step (see ``kv_shard.PeerOutput``)."""
-    import ctypes
     arr = (ctypes.c_void_p * len(flag_ptrs))(*[int(p) for p in flag_ptrs])
     rc = L.lib().mf_peer_barrier(arr, len(flag_ptrs), int(rank), int(epoch),
                                  err_word(device).data_ptr(), _stream_ptr(device))

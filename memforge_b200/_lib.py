@@ -46,6 +46,9 @@ EXPORTED = (
     "mf_paged_attention_workspace_size", "mf_paged_attention", "mf_paged_decode",
     "mf_copy_blocks", "mf_paged_decode_noalloc", "mf_peer_barrier", "mf_ipc_export",
     "mf_ipc_open", "mf_ipc_close", "mf_commit_window", "mf_gather_kv", "mf_accept_commit",
+    "mf_paged_attention_scored_workspace_size", "mf_paged_attention_scored",
+    "mf_q4_record_bytes", "mf_q4_reshape_and_cache", "mf_q4_gather_kv",
+    "mf_q4_paged_attention_workspace_size", "mf_q4_paged_attention",
 )
 
 MF_IPC_HANDLE_BYTES = 64
@@ -74,6 +77,30 @@ class AttentionArgs(ctypes.Structure):
         ("scale", c_f32), ("causal", c_i32), ("dtype", ctypes.c_int),
         ("num_out_peers", c_i32), ("out_head_offset", c_i32),
         ("out_peers", c_vp * MF_MAX_OUT_PEERS),
+    ]
+
+
+class ScoreMods(ctypes.Structure):
+    """Mirror of ``mf_score_mods``."""
+    _fields_ = [("softcap", c_f32), ("window", c_i32), ("alibi_slopes", c_vp),
+                ("prefix_lens", c_vp)]
+
+
+class Q4AttentionArgs(ctypes.Structure):
+    """Mirror of ``mf_q4_attention_args``."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("q", c_vp), ("q_stride_row", c_i64), ("q_stride_head", c_i64),
+        ("out", c_vp), ("out_stride_row", c_i64), ("out_stride_head", c_i64),
+        ("pool", c_vp), ("pool_stride_block", c_i64), ("pool_stride_head", c_i64),
+        ("num_blocks", c_i32),
+        ("block_tables", c_vp), ("table_stride", c_i32), ("table_width", c_i32),
+        ("cu_seqlens_q", c_vp), ("q_per_seq", c_i32),
+        ("kv_lens", c_vp), ("row_map", c_vp),
+        ("num_seqs", c_i32), ("total_q", c_i32), ("max_q_len", c_i32),
+        ("num_q_heads", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32),
+        ("scale", c_f32), ("causal", c_i32), ("dtype", ctypes.c_int),
+        ("mods", ScoreMods),
     ]
 
 
@@ -124,7 +151,6 @@ def _declare(lib):
         c_vp, c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, ctypes.c_int,
         c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]
     lib.mf_paged_attention_workspace_size.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_int]
-    lib.mf_paged_attention_workspace_size.restype = c_sz
     lib.mf_paged_attention.argtypes = [ctypes.POINTER(AttentionArgs), c_vp, c_sz, c_vp, c_vp]
     lib.mf_paged_decode.argtypes = [
         c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp, c_i32, c_vp, c_i32,
@@ -146,8 +172,27 @@ def _declare(lib):
     lib.mf_paged_decode_noalloc.argtypes = [
         c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp, c_i32, c_vp, c_i32,
         c_i32, c_i32, c_i32, c_i32, c_f32, ctypes.c_int, c_vp, c_vp, c_vp]
+    lib.mf_paged_attention_scored_workspace_size.argtypes = [
+        ctypes.POINTER(AttentionArgs), ctypes.POINTER(ScoreMods), ctypes.c_int]
+    lib.mf_paged_attention_scored.argtypes = [
+        ctypes.POINTER(AttentionArgs), ctypes.POINTER(ScoreMods), c_vp, c_sz, c_vp, c_vp]
+    lib.mf_q4_record_bytes.argtypes = [c_i32]
+    lib.mf_q4_reshape_and_cache.argtypes = [
+        c_vp, c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp,
+        c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]
+    lib.mf_q4_gather_kv.argtypes = [
+        c_vp, c_i64, c_i64, c_i32, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, ctypes.c_int,
+        c_i64, c_i64, c_vp, c_vp]
+    lib.mf_q4_paged_attention_workspace_size.argtypes = [ctypes.POINTER(Q4AttentionArgs),
+                                                         ctypes.c_int]
+    lib.mf_q4_paged_attention.argtypes = [ctypes.POINTER(Q4AttentionArgs), c_vp, c_sz, c_vp, c_vp]
+    sizes = ("mf_paged_attention_workspace_size", "mf_paged_attention_scored_workspace_size",
+             "mf_q4_paged_attention_workspace_size")
+    for name in sizes:
+        getattr(lib, name).restype = c_sz
+    lib.mf_q4_record_bytes.restype = c_i64
     for name in EXPORTED:
-        if name not in ("mf_last_error", "mf_paged_attention_workspace_size"):
+        if name not in sizes and name not in ("mf_last_error", "mf_q4_record_bytes"):
             getattr(lib, name).restype = ctypes.c_int
     return lib
 

@@ -65,7 +65,7 @@ def build(force: bool = False, ptxas_verbose: bool = False) -> str:
         with open(STAMP) as fh:
             if fh.read().strip() == digest:
                 return LIB
-    cmd = [nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-o", LIB + ".tmp", *sources()]
+    cmd = [nvcc(), "-t", "0", *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-o", LIB + ".tmp", *sources()]
     # Exported symbols: only the extern "C" mf_* API (everything else is hidden).
     cmd += ["-Xlinker", "--version-script=" + os.path.join(CSRC, "exports.map")]
     if ptxas_verbose:

@@ -21,7 +21,9 @@ constexpr int GEN_ROWS = 32;   // query rows per CTA
 constexpr int GEN_TILE = 32;   // keys per shared-memory tile
 constexpr int GEN_RPW = GEN_ROWS / GEN_WARPS;
 
-template <typename T, int DMAX>
+// MOD: modified scores (mf_score.cuh).  Keys left of a window that no row of the tile sees
+// are not loaded, and a row without a visible key is zeros, not an error.
+template <typename T, int DMAX, bool MOD>
 __global__ void __launch_bounds__(GEN_WARPS * 32)
     attn_generic_kernel(AttnParams p, int row_tiles) {
   constexpr int CPL = DMAX / 32;  // accumulator columns per lane
@@ -42,10 +44,10 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
   const T* q = static_cast<const T*>(p.q);
   T* out = static_cast<T*>(p.out);
 
-  if (kv_len < q_len || kv_len <= 0) {
+  if (MOD ? kv_len <= 0 : kv_len < q_len || kv_len <= 0) {
     // No visible key for some row: the reference raises (varlen_attention.py:
     // 228-232); here the rows are zeroed and the error word says why.
-    if (tid == 0) set_err(p.err, MF_ERR_LENGTH);
+    if (tid == 0 && (!MOD || kv_len < 0)) set_err(p.err, MF_ERR_LENGTH);
     for (int idx = tid; idx < (r1 - r0) * D; idx += blockDim.x) {
       const int r = r0 + idx / D, d = idx % D;
       const int prow = map_row(p, q_start + r / G);
@@ -55,7 +57,11 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
   }
   const int win_start = kv_len - q_len;
   const int last_i = (r1 - 1) / G;
-  const int key_end = (p.causal ? win_start + last_i : kv_len - 1) + 1;
+  const int pfx = MOD && p.mods.prefix ? min(max(p.mods.prefix[s], 0), kv_len) : 0;
+  const int key_end = max((p.causal ? win_start + last_i : kv_len - 1) + 1, pfx);
+  // First key that the tile's first row sees through the window.
+  const int key_lo =
+      MOD && p.mods.window > 0 ? max(win_start + r0 / G - p.mods.window + 1, 0) : 0;
 
   extern __shared__ float gsm[];
   float* sq = gsm;                             // [GEN_ROWS][D]
@@ -85,6 +91,7 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
   const float scale = p.scale;
 
   for (int t0 = 0; t0 < key_end; t0 += GEN_TILE) {
+    if (MOD && t0 >= pfx && t0 + GEN_TILE <= key_lo) continue;
     // Resolve each key of the tile to an element offset: >= 0 pool offset,
     // -2 - row for a window row, -1 for nothing (past the range / bad id).
     if (tid < GEN_TILE) {
@@ -135,13 +142,23 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
       const int i = r / G;
       const int limit = p.causal ? win_start + i : kv_len - 1;
       const int kpos = t0 + lane;
+      bool see = kpos <= limit;
+      if (MOD) {
+        if (p.mods.window > 0) see = see && win_start + i - kpos < p.mods.window;
+        see = (see || kpos < pfx) && kpos < kv_len;
+      }
       float sc = -INFINITY;
-      if (kpos <= limit) {
+      if (see) {
         float dot = 0.f;
         const float* qr = sq + rr * D;
         const float* kr = sk + lane * (D + 1);
         for (int d = 0; d < D; ++d) dot = fmaf(qr[d], kr[d], dot);
         sc = dot * scale;
+        if (MOD) {
+          if (p.mods.softcap > 0.f) sc = p.mods.softcap * tanhf(sc / p.mods.softcap);
+          if (p.mods.slopes)
+            sc = fmaf(-p.mods.slopes[h * G + r % G], (float)(win_start + i - kpos), sc);
+        }
       }
       float tmax = sc;
 #pragma unroll
@@ -149,16 +166,18 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
       const float m_new = fmaxf(m[k], tmax);
       if (m_new == -INFINITY) continue;  // nothing visible yet (cannot happen past tile 0)
       const float alpha = (m[k] == -INFINITY) ? 0.f : expf(m[k] - m_new);
-      const float pj = (kpos <= limit) ? expf(sc - m_new) : 0.f;
+      const float pj = see ? expf(sc - m_new) : 0.f;
       float psum = pj;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) psum += __shfl_xor_sync(0xffffffffu, psum, o);
       l[k] = l[k] * alpha + psum;
 #pragma unroll
       for (int c = 0; c < CPL; ++c) acc[k][c] *= alpha;
-      const int nvis = min(GEN_TILE, limit - t0 + 1);
+      const int nvis = min(GEN_TILE, (MOD ? key_end - 1 : limit) - t0 + 1);
+      const uint32_t seen = MOD ? __ballot_sync(0xffffffffu, see) : 0xffffffffu;
       for (int j = 0; j < nvis; ++j) {
         const float pb = __shfl_sync(0xffffffffu, pj, j);
+        if (MOD && !((seen >> j) & 1u)) continue;  // a value the row does not see may be NaN
 #pragma unroll
         for (int c = 0; c < CPL; ++c) {
           const int d = lane + 32 * c;
@@ -192,14 +211,15 @@ static int launch_gen(const AttnParams& p, cudaStream_t stream) {
   const int64_t gx = (int64_t)p.num_seqs * row_tiles;
   if (gx == 0) return MF_OK;
   if (gx > 0x7fffffff) return fail(MF_EINVAL, "generic attention: grid too large");
+  auto kern = p.mods.any() ? attn_generic_kernel<T, DMAX, true> : attn_generic_kernel<T, DMAX, false>;
   const size_t smem = (size_t)(GEN_ROWS * p.d + 2 * GEN_TILE * (p.d + 1)) * sizeof(float) +
                       GEN_TILE * sizeof(int64_t);
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(attn_generic_kernel<T, DMAX>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
     if (e != cudaSuccess) return fail(MF_ECUDA, std::string("generic attention: ") + cudaGetErrorString(e));
   }
-  attn_generic_kernel<T, DMAX><<<dim3((unsigned)gx, p.hkv), GEN_WARPS * 32, smem, stream>>>(p, row_tiles);
+  kern<<<dim3((unsigned)gx, p.hkv), GEN_WARPS * 32, smem, stream>>>(p, row_tiles);
   return check_launch("paged attention (generic)");
 }
 

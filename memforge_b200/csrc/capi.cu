@@ -203,6 +203,41 @@ extern "C" int mf_paged_attention(const mf_attention_args* args, void* workspace
   return launch_attn_tc(d.short_p, args->dtype, d.decode, workspace, s);
 }
 
+// Modified scores are served by the generic kernel.
+static int to_scored(const mf_attention_args* args, const mf_score_mods* mods, int32_t* err,
+                     AttnParams& p) {
+  const int rc = to_params(args, err, p);
+  if (rc != MF_OK) return rc;
+  if (!mods) return fail(MF_EINVAL, "scored attention: null mods");
+  if (!(mods->softcap >= 0.f) || mods->softcap > 1e30f || mods->window < 0)
+    return fail(MF_EINVAL, "scored attention: softcap and window must not be negative");
+  p.mods = {mods->softcap, mods->alibi_slopes, mods->window, mods->prefix_lens};
+  if (p.mods.any() && (p.wk || p.n_peers > 0))
+    return fail(MF_EUNSUPPORTED, "scored attention: a side window or peer output is not served "
+                                 "with score modifiers");
+  return MF_OK;
+}
+
+extern "C" size_t mf_paged_attention_scored_workspace_size(const mf_attention_args* args,
+                                                           const mf_score_mods* mods,
+                                                           int device) {
+  AttnParams p{};
+  if (to_scored(args, mods, nullptr, p) != MF_OK) return 0;
+  if (!p.mods.any()) return mf_paged_attention_workspace_size(args, device);
+  return 0;
+}
+
+extern "C" int mf_paged_attention_scored(const mf_attention_args* args, const mf_score_mods* mods,
+                                         void* workspace, size_t workspace_bytes,
+                                         int32_t* err_flag, mf_stream_t stream) {
+  AttnParams p{};
+  const int rc = to_scored(args, mods, err_flag, p);
+  if (rc != MF_OK) return rc;
+  if (!p.mods.any()) return mf_paged_attention(args, workspace, workspace_bytes, err_flag, stream);
+  if (p.num_seqs == 0 || p.total_q == 0) return MF_OK;
+  return launch_attn_generic(p, args->dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
 extern "C" int mf_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h,
                                const void* key_flat, const void* value_flat,
                                int64_t flat_stride_slot, int64_t flat_stride_head,

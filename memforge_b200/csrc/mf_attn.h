@@ -3,6 +3,7 @@
 #pragma once
 
 #include "mf_internal.h"
+#include "mf_score.cuh"
 
 namespace mf {
 
@@ -34,6 +35,7 @@ struct AttnParams {
   int32_t n_peers;
   int32_t out_head_offset;
   void* out_peers[MF_MAX_OUT_PEERS];
+  ScoreMods mods;  // all zero: plain scores
 };
 
 // Output targets of a call (the peers' buffers, or `out`) and the address of

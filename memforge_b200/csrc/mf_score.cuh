@@ -1,0 +1,40 @@
+// Modified attention scores: capped, biased by distance, windowed, with a prefix.
+#pragma once
+
+#include "mf_internal.h"
+
+namespace mf {
+
+// Score modifiers, in this order: s = scale q.k; softcap > 0: s = softcap *
+// tanh(s / softcap); slopes: s -= slopes[query head] * (query position - key
+// position); then the mask.  Key k is visible to the row at position p iff
+// k < kv_len and (k < prefix or ((not causal or k <= p) and (window == 0 or
+// p - k < window))).
+struct ScoreMods {
+  float softcap;
+  const float* slopes;    // [num_q_heads] or null
+  int32_t window;         // 0: none
+  const int32_t* prefix;  // [num_seqs] or null
+  __host__ __device__ bool any() const {
+    return softcap > 0.f || slopes != nullptr || window > 0 || prefix != nullptr;
+  }
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+MF_DEVINL float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap * tanh(s / cap) with score and result in log2 units: cap2 = cap * log2(e),
+// two_over = 2 / cap (s2 = s * log2 e, so exp(2 s / cap) = 2^(s2 * 2 / cap)).
+// From tanh(y) = 1 - 2 / (1 + exp(2y)): absolute error about cap2 * 2^-23, where the
+// hardware's own tanh (relative 2^-11) would move a weight by cap * 2^-11.  An
+// overflowing exponential gives rcp(inf) = 0, the cap itself.
+MF_DEVINL float softcap_log2(float s2, float cap2, float two_over) {
+  return fmaf(-2.f * cap2, rcp_approx(1.f + fast_exp2(s2 * two_over)), cap2);
+}
+
+}  // namespace mf
