@@ -422,6 +422,10 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
   for (int it = 0; it < C.max_len; ++it, stage = (stage + 1 == NS) ? 0 : stage + 1,
            phase ^= (stage == 0) ? 1u : 0u) {
     if (it >= len) {
+      // No page of mine in this stage.  Still wait for it: released at once, this warp
+      // could run a whole ring ahead and arrive twice for one use of the stage, in place
+      // of a warp that is still reading.
+      if (!wait_full(C, stage, phase)) return;
       release(C, stage);
       continue;
     }
@@ -638,6 +642,10 @@ MF_DEVINL void consume_split(const Ctx& C) {
   for (int it = 0; it < C.max_len; ++it, stage = (stage + 1 == NS) ? 0 : stage + 1,
            phase ^= (stage == 0) ? 1u : 0u) {
     if (it >= len) {
+      // No page of mine in this stage.  Still wait for it: released at once, this warp
+      // could run a whole ring ahead and arrive twice for one use of the stage, in place
+      // of a warp that is still reading.
+      if (!wait_full(C, stage, phase)) return;
       release(C, stage);
       continue;
     }

@@ -73,6 +73,18 @@ def test_one_or_two_kv_heads_many_ranges(hq, hkv):
     check(c)
 
 
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (8, 2), (16, 4)])
+def test_idle_ranges_beside_busy_ones(hq, hkv):
+    """Few pages for a GPU whose CTAs run several ranges each: ranges without a page share
+    a CTA's ring with ranges of more pages than the ring has stages, and must not free a
+    stage that is still being read."""
+    for ctx in ([1, 20, 40, 30], [70], [100, 17], [64, 64], [1, 100]):
+        c = cases.small_decode_case(f"idle{hkv}", 24, "bf16", hq, hkv, 128, ctx)
+        want = cases.oracle_decode(c)
+        for _ in range(20):
+            assert_close(run_case(c), want, "bf16", c.name)
+
+
 def test_many_short_sequences():
     g = cases.rng(9)
     ctx = g.integers(1, 80, size=300).tolist()
