@@ -25,6 +25,10 @@
 //    the log2 domain with quad shuffles.
 //  * When fewer than 8 (head, m-tile, half) units exist, the CTA runs
 //    PPS = 8/units independent virtual CTAs side by side, one page each per stage.
+//  * MOD instances apply score modifiers (mf_score.cuh) to S^T / S before the softmax.
+//    Pages that no row of a sequence sees (behind the window and the prefix) are left
+//    out of the page list, so a window costs its own bytes: `gap` pages are skipped
+//    after the prefix's `pa` pages.
 //  * Every mbarrier wait is bounded; on expiry the CTA sets MF_ERR_TIMEOUT,
 //    drains its own TMA loads and returns.
 //
@@ -63,14 +67,16 @@ struct Smem {
   uint32_t page_bytes, stage_bytes, bar_off, prefix_off, qstart_off, flag_off, total;
 };
 
-__host__ __device__ inline Smem smem_layout(int D, int HG, int PPS, int NS, int B, int window) {
+// per_seq: bytes the producer keeps per sequence (its first row with a window, the
+// page gap with score modifiers, else nothing).
+__host__ __device__ inline Smem smem_layout(int D, int HG, int PPS, int NS, int B, int per_seq) {
   Smem s;
   s.page_bytes = (uint32_t)(HG * PAGE * D * 2);
   s.stage_bytes = 2u * PPS * s.page_bytes;
   s.bar_off = NS * s.stage_bytes;
   s.prefix_off = s.bar_off + 2 * NS * 8;
   s.qstart_off = s.prefix_off + (uint32_t)(B + 1) * 4;
-  s.flag_off = s.qstart_off + (window ? (uint32_t)B * 4 : 0u);
+  s.flag_off = s.qstart_off + (uint32_t)(per_seq * B);
   s.total = s.flag_off + 16;
   return s;
 }
@@ -88,13 +94,20 @@ MF_DEVINL uint32_t tile_addr(uint32_t base, int tok, int hl, int chunk) {
 // Page geometry of sequence i (identical in the prologue and the consumers).
 struct SeqGeo {
   int q_start, q_len, kv_len, pool_len, pool_pages, pages;
+  int pfx, pa, gap;  // MOD: prefix keys and pages, pages left out after them
+
+  template <bool MOD>
+  MF_DEVINL int page(int k) const { return !MOD || k < pa ? k : k + gap; }
 };
 
+template <bool MOD>
 MF_DEVINL SeqGeo seq_geo(const Params& P, int i) {
   SeqGeo g;
+  g.pfx = g.pa = g.gap = 0;
   seq_rows(P.a, i, g.q_start, g.q_len);
   g.kv_len = P.a.kv_lens[i];
-  const bool bad = g.q_len < 0 || g.kv_len < g.q_len || (g.q_len > 0 && g.kv_len <= 0) ||
+  const bool bad = g.q_len < 0 || (!MOD && g.kv_len < g.q_len) ||
+                   (g.q_len > 0 && g.kv_len <= 0) ||
                    g.q_len * P.G > P.rows_cap || (P.window && g.q_len > PAGE);
   if (bad || g.q_len == 0) {
     g.pool_len = 0;
@@ -105,6 +118,15 @@ MF_DEVINL SeqGeo seq_geo(const Params& P, int i) {
   g.pool_len = P.window ? g.kv_len - g.q_len : g.kv_len;
   g.pool_pages = (g.pool_len + PAGE - 1) / PAGE;
   if (g.pool_pages > P.a.table_stride) g.pool_pages = P.a.table_stride;  // flagged in prologue
+  if (MOD) {
+    if (P.a.mods.prefix) g.pfx = min(max(P.a.mods.prefix[i], 0), g.kv_len);
+    g.pa = min((g.pfx + PAGE - 1) / PAGE, g.pool_pages);
+    const int lo =
+        P.a.mods.window > 0 ? max(g.kv_len - g.q_len - P.a.mods.window + 1, 0) : 0;
+    g.gap = max(min(lo / PAGE, g.pool_pages) - g.pa, 0);
+    g.pages = g.pool_pages - g.gap;
+    return g;
+  }
   g.pages = g.pool_pages + (P.window ? 1 : 0);
   return g;
 }
@@ -384,12 +406,44 @@ MF_DEVINL uint32_t movm_trans(uint32_t x) {
   return y;
 }
 
+// Score modifiers of one page: key positions and rows come as (key, query position).
+struct PageMods {
+  float cap2, two_over;
+  int window, pfx, kv_len, causal;
+  bool slopes;
+  MF_DEVINL explicit PageMods(const Params& P, const SeqGeo& g)
+      : cap2(P.a.mods.softcap * kLog2e),
+        two_over(2.f / P.a.mods.softcap),
+        window(P.a.mods.window),
+        pfx(g.pfx),
+        kv_len(g.kv_len),
+        causal(P.a.causal),
+        slopes(P.a.mods.slopes != nullptr) {}
+  // s: score in log2 units; slope in log2 units.
+  MF_DEVINL float score(float s, float slope, int back) const {
+    if (cap2 > 0.f) s = softcap_log2(s, cap2, two_over);
+    return slopes ? fmaf(-slope, (float)back, s) : s;
+  }
+  MF_DEVINL bool sees(int key, int qpos) const {
+    const bool see = (!causal || key <= qpos) && (window == 0 || qpos - key < window);
+    return (see || key < pfx) && key < kv_len;
+  }
+  // Whether some row (from query position first on) sees the key.
+  MF_DEVINL bool live(int key, int first) const {
+    return key < kv_len && (key < pfx || window == 0 || first - key < window);
+  }
+};
+
+MF_DEVINL float row_slope(const Params& P, int head, int r, int rows) {
+  return P.a.mods.slopes && r < rows ? P.a.mods.slopes[head * P.G + r % P.G] * kLog2e : 0.f;
+}
+
 // -------------------------------------------------------------------------
 // Consumer for up to 8 query rows per kv head (decode): one warp per kv head.
 // S^T = K Q^T (M = 16 tokens, N = 8 rows, K = head_dim), P^T turned into the B
 // operand with movmatrix, O^T = V^T P^T (M = head_dim in 16-row tiles).
 // -------------------------------------------------------------------------
-template <typename T, int D>
+template <typename T, int D, bool MOD>
 MF_DEVINL void consume_swapped(const Ctx& C) {
   const Params& P = C.P;
   using M = Mma<T>;
@@ -416,6 +470,7 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
   uint32_t qb[D / 16][2];   // Q^T as the B operand: (k = dims, n = row g4)
   float o[D / 16][4];       // O^T: (dims g4 / g4+8 of each 16-dim tile, rows 2c4, 2c4+1)
   float mrow[2], lrow[2];   // rows 2c4, 2c4+1
+  float slope[2] = {0.f, 0.f};
 
   int stage = 0;
   uint32_t phase = 0;
@@ -435,7 +490,7 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
       si = c.i;
       k = c.k;
       k0 = k;
-      geo = seq_geo(P, si);
+      geo = seq_geo<MOD>(P, si);
       const int head = hg * P.HG + hl;
       const int qi = g4 / P.G, gg = g4 % P.G;
       const bool valid = qi < geo.q_len;
@@ -449,6 +504,10 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
       }
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      if (MOD) {
+        slope[0] = row_slope(P, head, 2 * c4, geo.q_len * G);
+        slope[1] = row_slope(P, head, 2 * c4 + 1, geo.q_len * G);
+      }
       mrow[0] = mrow[1] = -INFINITY;
       lrow[0] = lrow[1] = 0.f;
     }
@@ -457,10 +516,15 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
     const uint32_t sK = C.base + stage * stage_bytes + ps * page_bytes;
     const uint32_t sV = sK + v_off;
     const bool is_win = window && k == geo.pool_pages;
-    const int kbase = is_win ? geo.pool_len : k * PAGE;
-    const int valid = is_win ? geo.q_len : min(PAGE, geo.pool_len - k * PAGE);
+    const int page = geo.template page<MOD>(k);
+    const int kbase = is_win ? geo.pool_len : page * PAGE;
+    const int valid = is_win ? geo.q_len : min(PAGE, geo.pool_len - page * PAGE);
     const int win_start = geo.kv_len - geo.q_len;
-    const bool need_mask = valid < PAGE || (causal && kbase + PAGE - 1 > win_start);
+    const PageMods pm(P, geo);
+    // MOD: the page starts behind the window of the last row (and ends past the prefix)
+    const bool left = MOD && pm.window > 0 && geo.kv_len - 1 - kbase >= pm.window &&
+                      kbase + PAGE > geo.pfx;
+    const bool need_mask = valid < PAGE || (causal && kbase + PAGE - 1 > win_start) || left;
 
     // S^T: two accumulators (even / odd k-steps) halve the dependent chain.
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -476,7 +540,12 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float v = (s0[e] + s1[e]) * sl2;
-      if (need_mask) {
+      if constexpr (MOD) {
+        const int key = kbase + g4 + 8 * (e >> 1);
+        const int qpos = win_start + (2 * c4 + (e & 1)) / G;
+        v = pm.score(v, slope[e & 1], qpos - key);
+        if (need_mask && !pm.sees(key, qpos)) v = -INFINITY;
+      } else if (need_mask) {
         const int tok = g4 + 8 * (e >> 1);
         const int r = 2 * c4 + (e & 1);
         const int lim = causal ? win_start + r / G : geo.kv_len - 1;
@@ -520,11 +589,15 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
       const int tok = (lane & 7) + ((lane >> 4) << 3);
       const int chunk = n * 2 + ((lane >> 3) & 1);
       ldsm_x4_trans(a[0], a[1], a[2], a[3], tile_addr<D>(sV, tok, hl, chunk));
-      if (valid < PAGE) {
-        // Unwritten slots may hold anything (NaN included): zero them.
+      if (valid < PAGE || left) {
+        // Unwritten slots may hold anything (NaN included): zero them, and with them
+        // the slots behind every row's window.
         const int t_lo = 2 * c4, t_hi = 8 + 2 * c4;
-        const uint32_t mlo = (t_lo < valid ? 0xffffu : 0u) | (t_lo + 1 < valid ? 0xffff0000u : 0u);
-        const uint32_t mhi = (t_hi < valid ? 0xffffu : 0u) | (t_hi + 1 < valid ? 0xffff0000u : 0u);
+        auto keep = [&](int t) {
+          return MOD ? pm.live(kbase + t, win_start) : t < valid;
+        };
+        const uint32_t mlo = (keep(t_lo) ? 0xffffu : 0u) | (keep(t_lo + 1) ? 0xffff0000u : 0u);
+        const uint32_t mhi = (keep(t_hi) ? 0xffffu : 0u) | (keep(t_hi + 1) ? 0xffff0000u : 0u);
         a[0] &= mlo;
         a[1] &= mlo;
         a[2] &= mhi;
@@ -605,7 +678,7 @@ MF_DEVINL void consume_swapped(const Ctx& C) {
 // (kv head, 16-row m-tile, half of head_dim); S = Q K^T in full, O[:, half] +=
 // P V.
 // -------------------------------------------------------------------------
-template <typename T, int D>
+template <typename T, int D, bool MOD>
 MF_DEVINL void consume_split(const Ctx& C) {
   const Params& P = C.P;
   using M = Mma<T>;
@@ -635,6 +708,7 @@ MF_DEVINL void consume_split(const Ctx& C) {
   uint32_t qf[D / 16][4];
   float o[DH / 8][4];
   float mrow[2], lrow[2];
+  float slope[2] = {0.f, 0.f};  // rows g4, g4 + 8 of the m-tile
 
   const int NS = P.NS;
   int stage = 0;
@@ -655,7 +729,7 @@ MF_DEVINL void consume_split(const Ctx& C) {
       si = c.i;
       k = c.k;
       k0 = k;
-      geo = seq_geo(P, si);
+      geo = seq_geo<MOD>(P, si);
       const int head = hg * P.HG + hl;
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2) {
@@ -678,6 +752,10 @@ MF_DEVINL void consume_split(const Ctx& C) {
       }
 #pragma unroll
       for (int n = 0; n < DH / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      if (MOD) {
+        slope[0] = row_slope(P, head, mt * 16 + g4, geo.q_len * P.G);
+        slope[1] = row_slope(P, head, mt * 16 + g4 + 8, geo.q_len * P.G);
+      }
       mrow[0] = mrow[1] = -INFINITY;
       lrow[0] = lrow[1] = 0.f;
     }
@@ -686,10 +764,14 @@ MF_DEVINL void consume_split(const Ctx& C) {
     const uint32_t sK = C.base + stage * C.L.stage_bytes + ps * C.L.page_bytes;
     const uint32_t sV = sK + P.PPS * C.L.page_bytes;
     const bool is_win = P.window && k == geo.pool_pages;
-    const int kbase = is_win ? geo.pool_len : k * PAGE;
-    const int valid = is_win ? geo.q_len : min(PAGE, geo.pool_len - k * PAGE);
+    const int page = geo.template page<MOD>(k);
+    const int kbase = is_win ? geo.pool_len : page * PAGE;
+    const int valid = is_win ? geo.q_len : min(PAGE, geo.pool_len - page * PAGE);
     const int win_start = geo.kv_len - geo.q_len;
-    const bool need_mask = valid < PAGE || (P.a.causal && kbase + PAGE - 1 > win_start);
+    const PageMods pm(P, geo);
+    const bool left = MOD && pm.window > 0 && geo.kv_len - 1 - kbase >= pm.window &&
+                      kbase + PAGE > geo.pfx;
+    const bool need_mask = valid < PAGE || (P.a.causal && kbase + PAGE - 1 > win_start) || left;
 
     float sc[2][4];
 #pragma unroll
@@ -709,7 +791,12 @@ MF_DEVINL void consume_split(const Ctx& C) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float s = sc[n][e] * sl2;
-        if (need_mask) {
+        if constexpr (MOD) {
+          const int key = kbase + n * 8 + 2 * c4 + (e & 1);
+          const int qpos = win_start + (mt * 16 + g4 + 8 * (e >> 1)) / P.G;
+          s = pm.score(s, slope[e >> 1], qpos - key);
+          if (need_mask && !pm.sees(key, qpos)) s = -INFINITY;
+        } else if (need_mask) {
           const int tok = n * 8 + 2 * c4 + (e & 1);
           const int r = mt * 16 + g4 + 8 * (e >> 1);
           const int lim = P.a.causal ? win_start + r / P.G : geo.kv_len - 1;
@@ -745,10 +832,13 @@ MF_DEVINL void consume_split(const Ctx& C) {
       const int tok = (lane & 7) + (((lane >> 3) & 1) << 3);
       const int chunk = dh * (DH / 8) + np * 2 + (lane >> 4);
       ldsm_x4_trans(b0, b1, b2, b3, tile_addr<D>(sV, tok, hl, chunk));
-      if (valid < PAGE) {
+      if (valid < PAGE || left) {
         const int t_lo = 2 * c4, t_hi = 8 + 2 * c4;
-        const uint32_t mlo = (t_lo < valid ? 0xffffu : 0u) | (t_lo + 1 < valid ? 0xffff0000u : 0u);
-        const uint32_t mhi = (t_hi < valid ? 0xffffu : 0u) | (t_hi + 1 < valid ? 0xffff0000u : 0u);
+        auto keep = [&](int t) {
+          return MOD ? pm.live(kbase + t, win_start) : t < valid;
+        };
+        const uint32_t mlo = (keep(t_lo) ? 0xffffu : 0u) | (keep(t_lo + 1) ? 0xffff0000u : 0u);
+        const uint32_t mhi = (keep(t_hi) ? 0xffffu : 0u) | (keep(t_hi + 1) ? 0xffff0000u : 0u);
         b0 &= mlo;
         b1 &= mhi;
         b2 &= mlo;
@@ -823,7 +913,7 @@ MF_DEVINL void consume_split(const Ctx& C) {
   }
 }
 
-template <typename T, int D, bool SW>
+template <typename T, int D, bool SW, bool MOD>
 __global__ void __launch_bounds__(THREADS, 1) decode_kernel(
     const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
     const __grid_constant__ CUtensorMap twk, const __grid_constant__ CUtensorMap twv,
@@ -833,7 +923,7 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(
   const uint32_t base = (raw_base + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw_base);
   const int B = P.a.num_seqs;
-  const Smem L = smem_layout(D, P.HG, P.PPS, P.NS, B, P.window);
+  const Smem L = smem_layout(D, P.HG, P.PPS, P.NS, B, P.window ? 4 : MOD ? 8 : 0);
   uint64_t* full = reinterpret_cast<uint64_t*>(gbase + L.bar_off);
   uint64_t* empty = full + P.NS;
   int* prefix = reinterpret_cast<int*>(gbase + L.prefix_off);
@@ -857,13 +947,32 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(
   // nothing in global memory is read before this point.
   grid_dependency_wait();
   for (int i = tid; i < B; i += blockDim.x) {
-    const SeqGeo g = seq_geo(P, i);
+    const SeqGeo g = seq_geo<MOD>(P, i);
     const bool other = P.skip_long && g.q_len * P.G > P.rows_cap;
-    if (g.q_len > 0 && g.pages == 0 && !other) set_err(P.a.err, MF_ERR_LENGTH);
+    // MOD: a sequence without keys is no error (its rows are written as zeros below)
+    if (g.q_len > 0 && g.pages == 0 && !other &&
+        (!MOD || g.kv_len < 0 || g.q_len * P.G > P.rows_cap))
+      set_err(P.a.err, MF_ERR_LENGTH);
     if (g.pages > 0 && (g.pool_len + PAGE - 1) / PAGE > P.a.table_stride)
       set_err(P.a.err, MF_ERR_TABLE);
     prefix[i + 1] = g.pages;
     if (P.window) qstart[i] = g.q_start;
+    if (MOD) {
+      qstart[2 * i] = g.pa;
+      qstart[2 * i + 1] = g.gap;
+    }
+  }
+  if constexpr (MOD) {
+    for (int i = blockIdx.x; i < B; i += gridDim.x) {
+      int q_start, q_len;
+      seq_rows(P.a, i, q_start, q_len);
+      if (P.a.kv_lens[i] > 0 || q_len <= 0 || q_len * P.G > P.rows_cap) continue;
+      for (int64_t e = tid; e < (int64_t)q_len * P.a.hq * D; e += blockDim.x) {
+        const int64_t r = e / D;
+        static_cast<T*>(P.a.out)[(int64_t)map_row(P.a, q_start + (int)(r / P.a.hq)) * P.a.o_sr +
+                                 (r % P.a.hq) * P.a.o_sh + e % D] = from_f32<T>(0.f);
+      }
+    }
   }
   __syncthreads();
   if (warp == 0) {
@@ -909,7 +1018,9 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(
     const int len = feeder ? S.len(vc) : 0;
     auto block_of = [&](const Cursor& c) -> int {
       if (P.window && c.k == c.pages - 1) return 0;  // window page: no table entry
-      return __ldg(P.a.tables + (int64_t)c.i * P.a.table_stride + c.k);
+      int page = c.k;
+      if (MOD && page >= qstart[2 * c.i]) page += qstart[2 * c.i + 1];
+      return __ldg(P.a.tables + (int64_t)c.i * P.a.table_stride + page);
     };
     Cursor cur{0, 0, 0, 1}, ahead{0, 0, 0, 1};
     int blk0 = 0, blk1 = 0;
@@ -978,9 +1089,9 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(
   if (warp >= active_warps) return;
   Ctx C{P, L, base, full, empty, abort_flag, prefix, B, T1, S, warp, lane, max_len};
   if constexpr (SW)
-    consume_swapped<T, D>(C);
+    consume_swapped<T, D, MOD>(C);
   else
-    consume_split<T, D>(C);
+    consume_split<T, D, MOD>(C);
 }
 
 }  // namespace tc
@@ -1035,7 +1146,8 @@ TcPlan plan_attn_tc(const AttnParams& p, mf_dtype dtype, int sm_count, bool wind
   if (sem_bytes > tc::SEM_REGION) return no("too many (sequence, head) counters");
   const int budget = 227 * 1024 - 1024;  // opt-in maximum minus alignment slack
   auto layout = [&](int ns) {
-    return tc::smem_layout(p.d, pl.HG, pl.PPS, ns, p.num_seqs, window ? 1 : 0);
+    return tc::smem_layout(p.d, pl.HG, pl.PPS, ns, p.num_seqs,
+                           window ? 4 : p.mods.any() ? 8 : 0);
   };
   int ns = 8;
   while (ns > 2 && layout(ns).total > (uint32_t)budget) --ns;
@@ -1091,16 +1203,19 @@ static int launch_tc_t(const AttnParams& p, const TcPlan& pl, void* ws, cudaStre
   P.sems = static_cast<int32_t*>(ws);
   P.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + tc::SEM_REGION);
   P.part_floats = (int)pl.part_floats;
-  auto kern = pl.SW ? tc::decode_kernel<T, D, true> : tc::decode_kernel<T, D, false>;
-  static thread_local int configured_dev[2] = {-1, -1};
+  const bool mod = p.mods.any();
+  auto kern = mod ? (pl.SW ? tc::decode_kernel<T, D, true, true> : tc::decode_kernel<T, D, false, true>)
+                  : (pl.SW ? tc::decode_kernel<T, D, true, false> : tc::decode_kernel<T, D, false, false>);
+  static thread_local int configured_dev[4] = {-1, -1, -1, -1};
+  const int which = pl.SW + 2 * mod;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (configured_dev[pl.SW] != dev) {
+  if (configured_dev[which] != dev) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          227 * 1024);
     if (e != cudaSuccess)
       return fail(MF_ECUDA, std::string("paged attention: ") + cudaGetErrorString(e));
-    configured_dev[pl.SW] = dev;
+    configured_dev[which] = dev;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)pl.ctas);

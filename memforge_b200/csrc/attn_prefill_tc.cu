@@ -41,6 +41,13 @@
 // load as zeros (out-of-range TMA coordinates) and unwritten slots of the last
 // page are zeroed in shared memory before the P V product.
 //
+// MOD instances apply score modifiers (mf_score.cuh) to S as it is read from TMEM.  Key
+// tiles that no row of a query tile sees (between the prefix and the window) are left
+// out, and so are the pages of a tile that lie behind the window.  The cap is a
+// polynomial while a warp's scores stay below 3/4 of it (3.5 packed instructions per
+// score, where the exponential and the reciprocal would add two SFU operations to the
+// softmax's one), else softcap_log2.
+//
 // Every mbarrier wait is bounded; on expiry the CTA raises MF_ERR_TIMEOUT, drains
 // its TMA loads and MMAs, frees its TMEM and returns.
 
@@ -152,6 +159,15 @@ struct Params {
 struct Item {
   int s, h, q_start, q_len, kv_len, win_start, pos0, nt;
   int pool_len;  // keys read from the pool (the rest, with a window, from the window buffers)
+  int pfx, pt, gap, lo;  // MOD: prefix keys and tiles, tiles left out after them, first
+                         // key that row 0 of the tile sees through the window
+
+  template <bool MOD>
+  MF_DEVINL int tile(int j) const { return !MOD || j < pt ? j : j + gap; }
+  template <bool MOD>
+  MF_DEVINL bool page_live(int page) const {
+    return !MOD || page * PAGE + PAGE - 1 >= lo || page * PAGE < pfx;
+  }
 };
 
 // Query positions per tile: the tile's rows are (position, query head) pairs,
@@ -169,6 +185,7 @@ MF_DEVINL int find_tile_seq(const int* prefix, int B, int t) {
 
 // Items run longest first: sequences by decreasing kv_len, and within a
 // sequence the last query tiles (which see the most keys) first.
+template <bool MOD>
 MF_DEVINL Item item_at(const Params& P, const int* prefix, const uint16_t* order, int B,
                        int it) {
   Item I;
@@ -184,7 +201,17 @@ MF_DEVINL Item item_at(const Params& P, const int* prefix, const uint16_t* order
   const int ppt = positions_per_tile(P.G);
   I.pos0 = qt * ppt;
   const int pos_last = min(I.q_len - 1, I.pos0 + ppt - 1);
-  if (P.window) {
+  I.pfx = I.pt = I.gap = I.lo = 0;
+  if constexpr (MOD) {
+    const ScoreMods& md = P.a.mods;
+    if (md.prefix) I.pfx = min(max(__ldg(md.prefix + I.s), 0), I.kv_len);
+    if (md.window > 0) I.lo = max(I.win_start + I.pos0 - md.window + 1, 0);
+    I.pool_len = I.kv_len;
+    I.pt = (I.pfx + BN - 1) / BN;
+    const int all = (max(I.win_start + pos_last + 1, I.pfx) + BN - 1) / BN;
+    I.gap = max(min(I.lo / BN, all) - I.pt, 0);
+    I.nt = max(all - I.gap, 1);  // a tile without any key still writes its rows
+  } else if (P.window) {
     // Pool tiles for positions < kv_len - q_len, then one tile holding the
     // window (q_len <= 16 keys) in its first rows.
     I.pool_len = I.win_start;
@@ -197,7 +224,48 @@ MF_DEVINL Item item_at(const Params& P, const int* prefix, const uint16_t* order
   return I;
 }
 
-template <typename T>
+// tanh(y) / y as a polynomial in y^2: least maximum of |tanh| error over |y| <= 3/4
+// (Lawson's reweighted least squares), 1.9e-7.
+constexpr float CAP_POLY_MAX = 0.75f;
+constexpr float CAP_POLY[5] = {0.9999972283095431f, -0.33323076454511924f, 0.1322609142435701f,
+                               -0.04928044211128824f, 0.01231882752544035f};
+
+// sv = capped scores in log2 units, of raw scores (times sl2: log2 units).
+template <int N>
+MF_DEVINL void cap_scores(float* sv, float sl2, float cap2) {
+  const float ky = sl2 / cap2;
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < N; c += 2)
+    top[(c >> 1) & 3] = fmax3f(top[(c >> 1) & 3], fabsf(sv[c]), fabsf(sv[c + 1]));
+  const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * ky;
+  if (__any_sync(0xffffffffu, mx > CAP_POLY_MAX)) {
+    const float two_over = 2.f / cap2;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const float s = sv[c] * sl2;
+      // exp(2 s / cap) = 2^(2 log2(e) s2 / cap2)
+      sv[c] = softcap_log2(s, cap2, two_over * kLog2e);
+    }
+  } else {
+    const uint64_t k2 = f32x2(ky, ky), s2 = f32x2(sl2, sl2);
+    const uint64_t c0 = f32x2(CAP_POLY[0], CAP_POLY[0]), c1 = f32x2(CAP_POLY[1], CAP_POLY[1]),
+                   c2 = f32x2(CAP_POLY[2], CAP_POLY[2]), c3 = f32x2(CAP_POLY[3], CAP_POLY[3]),
+                   c4 = f32x2(CAP_POLY[4], CAP_POLY[4]);
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const uint64_t v = f32x2(sv[c], sv[c + 1]);
+      const uint64_t y = f32x2_mul(v, k2), u = f32x2_mul(y, y);
+      uint64_t t = f32x2_fma(u, c4, c3);
+      t = f32x2_fma(u, t, c2);
+      t = f32x2_fma(u, t, c1);
+      t = f32x2_fma(u, t, c0);
+      f32x2_split(f32x2_mul(f32x2_mul(v, s2), t), sv[c], sv[c + 1]);
+    }
+  }
+}
+
+template <typename T, bool MOD>
 __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
     const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
     const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmwk,
@@ -258,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
     int tiles = 0;
     const int kvl = P.a.kv_lens[i];
     if (ql > 0 && ql * G > P.rows_cap) {
-      if (kvl < ql) {
+      if (MOD ? kvl < 0 : kvl < ql) {
         set_err(P.a.err, MF_ERR_LENGTH);
       } else if (((P.window ? kvl - ql : kvl) + PAGE - 1) / PAGE > P.a.table_stride) {
         set_err(P.a.err, MF_ERR_TABLE);
@@ -377,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
     for (int k = 0; run && snake_item(k) < items; ++k) {
       run = __shfl_sync(0xffffffffu, *abort_flag == 0, 0);
       if (!run) break;
-      const Item I = item_at(P, prefix, order, B, snake_item(k));
+      const Item I = item_at<MOD>(P, prefix, order, B, snake_item(k));
       if (!is_v) {
         const int qb = ic & 1;
         bool fine = true;
@@ -402,16 +470,19 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
       const int32_t* table = P.a.tables + (int64_t)I.s * P.a.table_stride;
       // Block id of this lane's page, loaded one tile ahead.  Out-of-table
       // pages use an out-of-range coordinate: TMA fills zeros.
-      int nxt = (boxer && my_pg < pool_pages) ? __ldg(table + my_pg) : -1;
+      auto block_of = [&](int page) {
+        return boxer && page < pool_pages && I.template page_live<MOD>(page) ? __ldg(table + page)
+                                                                             : -1;
+      };
+      int nxt = block_of(I.template tile<MOD>(0) * (BN / PAGE) + my_pg);
       for (int j = 0; j < I.nt; ++j, ++g) {
-        const int L = j * (BN / PAGE) + my_pg;
+        const int L = I.template tile<MOD>(j) * (BN / PAGE) + my_pg;
         int tok = nb * PAGE;
-        if (boxer && L < pool_pages) {
+        if (boxer && L < pool_pages && I.template page_live<MOD>(L)) {
           if (nxt >= 0 && nxt < nb) tok = nxt * PAGE;
           else set_err(P.a.err, MF_ERR_BLOCK_ID);
         }
-        if (j + 1 < I.nt)
-          nxt = (boxer && L + BN / PAGE < pool_pages) ? __ldg(table + L + BN / PAGE) : -1;
+        if (j + 1 < I.nt) nxt = block_of(I.template tile<MOD>(j + 1) * (BN / PAGE) + my_pg);
         const int st = g % KS;
         // With a window, the last tile is the window: 16 rows of each half.
         const bool win_tile = P.window && j == I.nt - 1;
@@ -461,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
       uint32_t g = 0;
       int ic = 0;
       for (int k = 0; ok && snake_item(k) < items; ++k, ++ic) {
-        const Item I = item_at(P, prefix, order, B, snake_item(k));
+        const Item I = item_at<MOD>(P, prefix, order, B, snake_item(k));
         const int qb = ic & 1;
         if (!is_pv) ok = mbar_wait_bounded(&bar[B_QFULL + qb], (ic >> 1) & 1, WAIT_LIMIT);
         const uint32_t qbase = base + OFF_Q + qb * TILE_BYTES;
@@ -531,7 +602,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
     float* mbox = reinterpret_cast<float*>(gbase + OFF_XCH);  // [2][BM]
     float* lbox = mbox + 2 * BM;                               // [2 items][2][BM]
     float* msbox = lbox + 4 * BM;                              // [2 items][2][BM]
-    const float sl2 = P.scale_log2;
+    // Scores that were capped or biased are in log2 units already.
+    const bool transformed = MOD && (P.a.mods.softcap > 0.f || P.a.mods.slopes);
+    const float sl2 = transformed ? 1.f : P.scale_log2;
     bool ok = true;
     // An item's epilogue runs after this warp's first tile of the next item
     // (or at the next item's end when it has none): by then the item's last
@@ -585,13 +658,16 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
     uint32_t g = 0;
     int ic = 0;
     for (int k = 0; ok && snake_item(k) < items; ++k, ++ic) {
-      const Item I = item_at(P, prefix, order, B, snake_item(k));
+      const Item I = item_at<MOD>(P, prefix, order, B, snake_item(k));
       const int pos = I.pos0 + row / G;  // query position of this row within the sequence
       const int gg = row % G;
       const bool row_valid = row < positions_per_tile(G) * G && pos < I.q_len;
       // Last visible key: causal over the context; with a window, every pool key
       // and, in the window tile, window keys 0..pos.
       const int limit = P.window ? I.pool_len - 1 : min(I.win_start + pos, I.kv_len - 1);
+      const int row_lo =
+          MOD && P.a.mods.window > 0 ? I.win_start + pos - P.a.mods.window + 1 : 0;
+      const float slope = MOD && P.a.mods.slopes ? P.a.mods.slopes[I.h * G + gg] * kLog2e : 0.f;
       float m_seen = -INFINITY;  // reference max l_own is scaled to
       float l_own = 0.f;
       for (int j = 0; j < I.nt; ++j, ++g) {
@@ -615,8 +691,23 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
 
         // Row max of the raw scores over the visible columns (c <= limit).
         const bool win_tile = P.window && j == I.nt - 1;
-        const int lim = win_tile ? pos : limit - j * BN;
-        if (__any_sync(0xffffffffu, lim < CW - 1)) {
+        const int kbase = I.template tile<MOD>(j) * BN;
+        const int lim = win_tile ? pos : limit - kbase;
+        if constexpr (MOD) {
+          if (P.a.mods.softcap > 0.f) cap_scores<CW>(sv, P.scale_log2, P.a.mods.softcap * kLog2e);
+          if (P.a.mods.slopes) {
+            const float up = P.a.mods.softcap > 0.f ? 1.f : P.scale_log2;
+            const float at = slope * (float)(kbase - (I.win_start + pos));
+#pragma unroll
+            for (int c = 0; c < CW; ++c) sv[c] = fmaf(sv[c], up, fmaf(slope, (float)c, at));
+          }
+          const int lo_c = row_lo - kbase, pf_c = I.pfx - kbase;
+          if (__any_sync(0xffffffffu, !(pf_c >= CW || (lim >= CW - 1 && lo_c <= 0)))) {
+#pragma unroll
+            for (int c = 0; c < CW; ++c)
+              if (c >= pf_c && (c > lim || c < lo_c)) sv[c] = -INFINITY;
+          }
+        } else if (__any_sync(0xffffffffu, lim < CW - 1)) {
 #pragma unroll
           for (int c = 0; c < CW; ++c)
             if (c > lim) sv[c] = -INFINITY;
@@ -710,19 +801,26 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(
           }
           tmem_wait_st();
         }
-        const int kbase = j * BN;
         // Keys of this tile past the last one loaded: past the pool in the last
         // pool tile, past q_len in the window tile (whose other rows were never
         // written by this tile's loads).
         const int loaded = win_tile ? I.q_len : I.pool_len - kbase;
-        if (quarter == 0 && loaded < BN) {
+        // MOD: keys [dead0, dead1) lie behind every row's window.
+        const int dead0 = MOD ? max(I.pfx - kbase, 0) : 0;
+        const int dead1 = MOD ? min(I.lo - kbase, BN) : 0;
+        if (quarter == 0 && (loaded < BN || dead0 < dead1)) {
           // Zero the V rows of those keys (whole 128-byte rows of both halves)
           // so p = 0 adds nothing even where a slot holds NaN.  This warp's
           // P-full arrival orders it before P V.
           const int st = g % KS;
           if (!mbar_wait_bounded(&bar[B_VFULL + st], (g / KS) & 1, WAIT_LIMIT)) ok = false;
           const uint32_t vb = base + OFF_V + st * TILE_BYTES;
-          const int first = max(0, loaded);
+          const int first = min(max(0, loaded), BN);
+          for (int idx = lane; MOD && idx < (dead1 - dead0) * 16; idx += 32) {
+            const int r = dead0 + idx / 16, c16 = idx % 16;
+            const uint32_t a = vb + (c16 >> 3) * HALF_BYTES + r * 128 + (c16 & 7) * 16;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
+          }
           for (int idx = lane; idx < (BN - first) * 16; idx += 32) {
             const int r = first + idx / 16, c16 = idx % 16;
             const uint32_t a = vb + (c16 >> 3) * HALF_BYTES + r * 128 + (c16 & 7) * 16;
@@ -878,12 +976,15 @@ int launch_attn_prefill_tc(const AttnParams& p, mf_dtype dtype, int rows_cap,
   const int64_t items_max = (int64_t)p.num_seqs * q_tiles * p.hkv;
   if (items_max == 0) return MF_OK;
   const int64_t grid = std::min<int64_t>(items_max, current_sm_count());
-  auto kern = dtype == MF_BF16 ? pf::prefill_kernel<__nv_bfloat16> : pf::prefill_kernel<__half>;
+  const bool mod = p.mods.any();
+  auto kern = dtype == MF_BF16
+                  ? (mod ? pf::prefill_kernel<__nv_bfloat16, true> : pf::prefill_kernel<__nv_bfloat16, false>)
+                  : (mod ? pf::prefill_kernel<__half, true> : pf::prefill_kernel<__half, false>);
   const size_t smem = pf::smem_bytes(p.num_seqs) + 1024;
-  static thread_local int configured_dev[2] = {-1, -1};
+  static thread_local int configured_dev[4] = {-1, -1, -1, -1};
   int dev = 0;
   cudaGetDevice(&dev);
-  const int which = dtype == MF_BF16 ? 1 : 0;
+  const int which = (dtype == MF_BF16 ? 1 : 0) + (mod ? 2 : 0);
   if (configured_dev[which] != dev) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)(pf::smem_bytes(pf::MAX_SEQS) + 1024));

@@ -157,6 +157,29 @@ Dispatch plan_dispatch(const AttnParams& p, mf_dtype dtype, int sm_count) {
   return d;
 }
 
+static size_t workspace_bytes_of(const AttnParams& p, mf_dtype dtype, int device) {
+  const Dispatch d = plan_dispatch(p, dtype, sm_count_of(device));
+  return (d.mode == Dispatch::DECODE || d.mode == Dispatch::MIXED) ? d.decode.ws_bytes : 0;
+}
+
+static int run_attention(const AttnParams& p, mf_dtype dtype, void* workspace,
+                         size_t workspace_bytes, cudaStream_t s) {
+  if (p.num_seqs == 0 || p.total_q == 0) return MF_OK;
+  const Dispatch d = plan_dispatch(p, dtype, current_sm_count());
+  if (p.n_peers > 0 && d.mode != Dispatch::DECODE)
+    return fail(MF_EUNSUPPORTED, "paged attention: peer output (num_out_peers) is served for "
+                                 "decode batches only");
+  if (d.mode == Dispatch::GENERIC) return launch_attn_generic(p, dtype, s);
+  if (d.mode == Dispatch::PREFILL) return launch_attn_prefill_tc(p, dtype, 0, s);
+  if (!workspace || workspace_bytes < d.decode.ws_bytes)
+    return fail(MF_EWORKSPACE, "paged attention: workspace missing or smaller than "
+                               "mf_paged_attention_workspace_size()");
+  if (d.mode == Dispatch::DECODE) return launch_attn_tc(p, dtype, d.decode, workspace, s);
+  const int rc = launch_attn_prefill_tc(p, dtype, d.rows_cap, s);
+  if (rc != MF_OK) return rc;
+  return launch_attn_tc(d.short_p, dtype, d.decode, workspace, s);
+}
+
 }  // namespace mf
 
 using namespace mf;
@@ -177,8 +200,7 @@ extern "C" int mf_device_info(int device, int* num_sms, int* is_sm100) {
 extern "C" size_t mf_paged_attention_workspace_size(const mf_attention_args* args, int device) {
   AttnParams p{};
   if (to_params(args, nullptr, p) != MF_OK) return 0;
-  const Dispatch d = plan_dispatch(p, args->dtype, sm_count_of(device));
-  return (d.mode == Dispatch::DECODE || d.mode == Dispatch::MIXED) ? d.decode.ws_bytes : 0;
+  return workspace_bytes_of(p, args->dtype, device);
 }
 
 extern "C" int mf_paged_attention(const mf_attention_args* args, void* workspace,
@@ -186,24 +208,10 @@ extern "C" int mf_paged_attention(const mf_attention_args* args, void* workspace
   AttnParams p{};
   int rc = to_params(args, err_flag, p);
   if (rc != MF_OK) return rc;
-  if (p.num_seqs == 0 || p.total_q == 0) return MF_OK;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const Dispatch d = plan_dispatch(p, args->dtype, current_sm_count());
-  if (p.n_peers > 0 && d.mode != Dispatch::DECODE)
-    return fail(MF_EUNSUPPORTED, "paged attention: peer output (num_out_peers) is served for "
-                                 "decode batches only");
-  if (d.mode == Dispatch::GENERIC) return launch_attn_generic(p, args->dtype, s);
-  if (d.mode == Dispatch::PREFILL) return launch_attn_prefill_tc(p, args->dtype, 0, s);
-  if (!workspace || workspace_bytes < d.decode.ws_bytes)
-    return fail(MF_EWORKSPACE, "paged attention: workspace missing or smaller than "
-                               "mf_paged_attention_workspace_size()");
-  if (d.mode == Dispatch::DECODE) return launch_attn_tc(p, args->dtype, d.decode, workspace, s);
-  rc = launch_attn_prefill_tc(p, args->dtype, d.rows_cap, s);
-  if (rc != MF_OK) return rc;
-  return launch_attn_tc(d.short_p, args->dtype, d.decode, workspace, s);
+  return run_attention(p, args->dtype, workspace, workspace_bytes,
+                       reinterpret_cast<cudaStream_t>(stream));
 }
 
-// Modified scores are served by the generic kernel.
 static int to_scored(const mf_attention_args* args, const mf_score_mods* mods, int32_t* err,
                      AttnParams& p) {
   const int rc = to_params(args, err, p);
@@ -223,8 +231,7 @@ extern "C" size_t mf_paged_attention_scored_workspace_size(const mf_attention_ar
                                                            int device) {
   AttnParams p{};
   if (to_scored(args, mods, nullptr, p) != MF_OK) return 0;
-  if (!p.mods.any()) return mf_paged_attention_workspace_size(args, device);
-  return 0;
+  return workspace_bytes_of(p, args->dtype, device);
 }
 
 extern "C" int mf_paged_attention_scored(const mf_attention_args* args, const mf_score_mods* mods,
@@ -233,9 +240,8 @@ extern "C" int mf_paged_attention_scored(const mf_attention_args* args, const mf
   AttnParams p{};
   const int rc = to_scored(args, mods, err_flag, p);
   if (rc != MF_OK) return rc;
-  if (!p.mods.any()) return mf_paged_attention(args, workspace, workspace_bytes, err_flag, stream);
-  if (p.num_seqs == 0 || p.total_q == 0) return MF_OK;
-  return launch_attn_generic(p, args->dtype, reinterpret_cast<cudaStream_t>(stream));
+  return run_attention(p, args->dtype, workspace, workspace_bytes,
+                       reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mf_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h,
