@@ -43,6 +43,7 @@
 
 #include "mf_attn.h"
 #include "mf_q4.cuh"
+#include "q4_attn.h"
 
 namespace mf {
 namespace q4a {
@@ -812,7 +813,11 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
 
 namespace {
 
+// Rows per kv head up to which mma.sync keeps a run when the tcgen05 kernel could have it.
+constexpr int ROWS_CAP = 32;
+
 struct Plan {
+  bool chunks, tiles;  // launch the tcgen05 kernel; launch the mma.sync kernel
   int nt, ranges;
   int64_t rt;
   size_t prefix_bytes, ws_bytes;
@@ -922,8 +927,15 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
 }
 
 Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
-  Plan pl;
-  const int64_t rows = (int64_t)P.a.max_q_len * P.G;
+  Plan pl{};
+  int64_t rows = (int64_t)P.a.max_q_len * P.G;
+  pl.chunks = rows > ROWS_CAP && q4_prefill_serves(P.a, dt);
+  pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
+  if (!pl.tiles) return pl;
+  if (pl.chunks) {
+    P.rows_cap = ROWS_CAP;
+    rows = std::min<int64_t>(rows, ROWS_CAP);
+  }
   pl.nt = row_tile(rows, P.a.d, dt == MF_F32);
   pl.rt = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
   P.RT = (int)pl.rt;
@@ -966,14 +978,19 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
   if (rc != MF_OK) return rc;
   if (P.a.num_seqs == 0 || P.a.total_q == 0 || P.a.max_q_len == 0) return MF_OK;
   const Plan pl = make_plan(P, args->dtype, current_sm_count());
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (pl.rt * P.a.hkv > 0x7fffffffLL) return fail(MF_EUNSUPPORTED, "q4 attention: too many row tiles");
-  if (!workspace || workspace_bytes < pl.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 15))
+  if (pl.tiles && (!workspace || workspace_bytes < pl.ws_bytes ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail(MF_EWORKSPACE, "q4 attention: workspace missing, misaligned or smaller than "
                                "mf_q4_paged_attention_workspace_size()");
   P.prefix = static_cast<int64_t*>(workspace);
-  P.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.prefix_bytes);
+  if (pl.tiles) P.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.prefix_bytes);
   P.part_floats = pl.part_floats;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (pl.chunks) {
+    const int rc2 = launch_q4_prefill(P.a, P.width, P.vec, P.rows_cap, args->dtype, s);
+    if (rc2 != MF_OK || !pl.tiles) return rc2;
+  }
   return with_kernel(
       args->dtype, P.a.d, pl.nt, P.a.mods.any(), [&](auto kern) -> int {
         using Kn = decltype(kern);

@@ -117,7 +117,7 @@ def attention(q, k, v, scale, see, softcap=0.0, slopes=None, kv_len=None):
 HALF_ULP = {"bf16": 2.0 ** -9, "f16": 2.0 ** -12, "f32": 2.0 ** -25}
 
 
-def q4_tolerance(dtype, out, q, codes_size, key_size, scale):
+def q4_tolerance(dtype, out, q, codes_size, key_size, scale, chunk=False):
     """
     Bound of |kernel - exact| for attention over 4-bit rows, elementwise.
 
@@ -127,10 +127,15 @@ def q4_tolerance(dtype, out, q, codes_size, key_size, scale):
       largest 15 * scale + |base| of a V row, which bounds every |n * scale|, |base|;
     * a score's error delta moves a weight by exp(delta) - 1, at most 2 delta, on top and
       bottom of the quotient (4 delta in all): fp32 sums of D products and of their
-      pieces, D * 2^-24 of scale * sum|q| * key_size, and 2^-21 for the exponential.
+      pieces, D * 2^-24 of scale * sum|q| * key_size, and 2^-21 for the exponential;
+    * chunk: long runs read keys and values rounded to fp16 (2^-12 relative each): the
+      values add 2^-12 of their size, the keys 2^-12 of scale * sum|q| * key_size to delta.
     """
     p = 2.0 ** -23 if dtype == "f32" else 2.0 ** -12
     D = q.shape[-1]
     size = scale * np.abs(q).sum(-1, keepdims=True) * key_size
     delta = D * 2.0 ** -24 * size + 2.0 ** -21
+    if chunk:
+        p += 2.0 ** -12
+        delta = delta + 2.0 ** -12 * size
     return 2 * HALF_ULP[dtype] * np.abs(out) + (p + 4 * delta) * codes_size + 1e-30

@@ -108,7 +108,8 @@ class Case:
             # |n * scale| and |base| of a row are at most its largest value plus its
             # span; three times the largest magnitude bounds their sum
             outs.append(o)
-            tols.append(R.q4_tolerance(self.dtype, o, q, 3 * size, 3 * size, self.scale))
+            chunk = self.d == 128 and self.dtype != "f32" and ql * self.hq // self.hkv > 32
+            tols.append(R.q4_tolerance(self.dtype, o, q, 3 * size, 3 * size, self.scale, chunk))
         return np.concatenate(outs), np.concatenate(tols)
 
     def check(self, **kw):
@@ -280,6 +281,61 @@ def test_several_rows_per_sequence(dtype, hq, hkv, d, ql):
 
 def test_ragged_runs_and_empty_ones():
     Case(11, "bf16", 8, 2, 128, [50, 200, 33, 9, 70], [3, 60, 0, 9, 1]).check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,ql", [(8, 2, 33), (4, 4, 129), (28, 4, 50), (40, 1, 7),
+                                       (48, 2, 11), (128, 1, 3)])
+def test_long_runs(dtype, hq, hkv, ql):
+    """Row tiles of 128 with every GQA size, odd ones included; contexts around key tiles."""
+    Case(50 + ql, dtype, hq, hkv, 128, [ql, ql + 127, ql + 128, 700], [ql] * 4).check()
+
+
+def test_long_runs_non_causal_and_without_keys():
+    Case(51, "bf16", 4, 2, 128, [150, 9], [70] * 2, causal=False).check()
+    got = Case(52, "bf16", 4, 1, 128, [0, 20, 300], [60] * 3).check()
+    assert not got[:60].any() and not got[60:100].any() and got[100:120].any()
+
+
+def test_long_runs_many_items_per_sm():
+    """More (tile, head) items than SMs, ragged: every CTA walks several."""
+    g = rng(53)
+    ql = g.integers(40, 200, 40).tolist()
+    Case(53, "bf16", 16, 8, 128, [q + int(g.integers(0, 300)) for q in ql], ql).check()
+
+
+def test_long_runs_of_large_values_and_offsets():
+    """Rows near fp16's largest number, rows on a large offset, and tiny rows."""
+    c = Case(54, "bf16", 4, 2, 128, [200], [50], q_scale=1e-6)
+    par = c.pool[:, :, 16 * 128:].view(np.float16).reshape(-1, 2, 2, 16, 2)
+    scale = np.zeros_like(par[..., 0])
+    base = np.zeros_like(scale)
+    scale[..., 0::3], base[..., 0::3] = 8728.0, -65504.0   # codes reach 65416
+    scale[..., 1::3], base[..., 1::3] = 0.5, 60000.0
+    scale[..., 2::3], base[..., 2::3] = 2.0 ** -24, -2.0 ** -20
+    par[..., 0], par[..., 1] = scale, base
+    c.check()
+
+
+def test_long_runs_row_map_and_strides():
+    c = Case(55, "bf16", 4, 1, 128, [90, 120], [40, 33])
+    rows = 73
+    wide_q = torch.zeros((rows + 2, 4, 131), dtype=torch.bfloat16, device="cuda")
+    perm = torch.from_numpy(rng(55).permutation(rows).astype(np.int32)).cuda()
+    wide_q[perm.long(), :, 1:129] = c.q_dev
+    wide_o = torch.full((rows + 2, 4, 133), 5.0, dtype=torch.bfloat16, device="cuda")
+    c.run(q=wide_q[:, :, 1:129], out=wide_o[:, :, 2:130],
+          row_map=torch.cat([perm, torch.tensor([73, 74], dtype=torch.int32, device="cuda")]))
+    want, tol = c.want()
+    got = wide_o[perm.long(), :, 2:130].double().cpu().numpy()
+    assert (np.abs(got - want) <= tol).all()
+    assert (wide_o[rows:] == 5.0).all() and (wide_o[:, :, :2] == 5.0).all()
+
+
+@pytest.mark.parametrize("window", [1, 16, 127, 128, 129, 300])
+def test_long_runs_windows_around_tiles(window):
+    Case(56, "bf16", 4, 1, 128, [500, 217, 640], [200] * 3, window=window).check()
+    Case(57, "f16", 4, 1, 128, [500, 217, 640], [200] * 3, window=window, prefix=[130, 1, 600]).check()
 
 
 def test_many_ranges_join():
