@@ -112,8 +112,23 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     return ws
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)   # a tenth of current_stream()'s host time
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_err_ptrs: Dict[int, int] = {}
+
+
+def _err_ptr(device: torch.device) -> int:
+    p = _err_ptrs.get(device.index)
+    if p is None:
+        p = _err_ptrs[device.index] = err_word(device).data_ptr()
+    return p
 
 
 def _after(what: str, device: torch.device) -> None:
@@ -130,9 +145,11 @@ def _on(device: torch.device):
 
 
 def require_one_device(what: str, device: torch.device, *tensors) -> None:
-    require_cuda(what, *tensors)
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is None or (t.is_cuda and t.device == device):
+            continue
+        require_cuda(what, t)
+        if t.device != device:
             raise ValueError(f"{what}: tensors on {device} and {t.device}")
 
 
@@ -468,85 +485,126 @@ Q4_BLOCK = 16
 
 def q4_head_dim(pool: torch.Tensor) -> int:
     """head_dim of a 4-bit pool layer ``(blocks, kv_heads, 16 * D + 128)``, checked."""
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.stride(-1) != 1:
-        raise ValueError(f"a 4-bit pool layer is uint8 (blocks, kv_heads, 16 * D + 128) with "
-                         f"contiguous records, got {pool.dtype} {tuple(pool.shape)}")
-    d = (pool.shape[2] - 128) // 16
-    if d not in (64, 128, 256) or pool.shape[2] != 16 * d + 128:
-        raise ValueError(f"no head_dim of 64, 128 or 256 has records of {pool.shape[2]} bytes")
-    return d
+    return _q4_layer(pool, None)[5]
+
+
+def _q4_layer(pool: torch.Tensor, layer: Optional[int]):
+    """(address, block stride, head stride, blocks, kv heads, head_dim) of one layer of a
+    4-bit pool ``([layers,] blocks, kv_heads, 16 * D + 128)``, without a view of it."""
+    shape, stride = pool.shape, pool.stride()
+    want = 3 if layer is None else 4
+    if pool.dtype != torch.uint8 or len(shape) != want or stride[-1] != 1:
+        raise ValueError(f"a 4-bit pool is uint8 ({'' if layer is None else 'layers, '}blocks, "
+                         f"kv_heads, 16 * D + 128) with contiguous records, got {pool.dtype} "
+                         f"{tuple(shape)}")
+    d = (shape[-1] - 128) // 16
+    if d not in (64, 128, 256) or shape[-1] != 16 * d + 128:
+        raise ValueError(f"no head_dim of 64, 128 or 256 has records of {shape[-1]} bytes")
+    ptr = pool.data_ptr()
+    if layer is not None:
+        if not -shape[0] <= layer < shape[0]:
+            raise IndexError(f"layer {layer} of a pool of {shape[0]}")
+        ptr += (layer % shape[0]) * stride[0]
+    return ptr, stride[-3], stride[-2], shape[-3], shape[-2], d
 
 
 def _slots(name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
+    if t.dtype != torch.int64 and t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32 or int64")
-    return t.reshape(-1).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def q4_reshape_and_cache(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor,
-                         slot_mapping: torch.Tensor) -> None:
+                         slot_mapping: torch.Tensor, *, layer: Optional[int] = None,
+                         heads_first: bool = False) -> None:
     """
     ``mf_q4_reshape_and_cache``: quantise ``key``/``value`` rows ``(T, H, D)`` (fp32,
     fp16 or bf16, any token and head strides) into one 4-bit pool layer
-    ``(blocks, H, 16 * D + 128)`` at ``slot_mapping[t]`` (-1 = skip).
+    ``(blocks, H, 16 * D + 128)`` at ``slot_mapping[t]`` (-1 = skip).  ``layer``: that
+    layer of a pool ``(layers, blocks, H, 16 * D + 128)``.  ``heads_first``: rows come as
+    ``(1, H, T, D)``.
     """
     dev = pool.device
     require_one_device("q4_reshape_and_cache", dev, pool, key, value, slot_mapping)
-    D = q4_head_dim(pool)
-    if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
-        raise ValueError(f"keys/values must be (T, H, D) of one shape and dtype, got "
-                         f"{tuple(key.shape)} {key.dtype} and {tuple(value.shape)} {value.dtype}")
-    T, H, d = key.shape
-    if (H, d) != (pool.shape[1], D):
-        raise ValueError(f"pool holds {pool.shape[1]} heads x {D} dims, keys are {H} x {d}")
-    if key.stride(-1) != 1:
+    ptr, sb, sh, nb, ph, D = _q4_layer(pool, layer)
+    shape = key.shape
+    if value.shape != shape or value.dtype != key.dtype or len(shape) != (4 if heads_first else 3):
+        raise ValueError(f"keys/values must be {'(1, H, T, D)' if heads_first else '(T, H, D)'} of "
+                         f"one shape and dtype, got {tuple(shape)} {key.dtype} and "
+                         f"{tuple(value.shape)} {value.dtype}")
+    ks, vs = key.stride(), value.stride()
+    if ks[-1] != 1:
         key = key.contiguous()
-    if value.stride(-1) != 1:
+        ks = key.stride()
+    if vs[-1] != 1:
         value = value.contiguous()
+        vs = value.stride()
+    if heads_first:
+        one, H, T, d = shape
+        if one != 1:
+            raise ValueError(f"keys/values must be (1, heads, tokens, head_dim), got "
+                             f"{tuple(shape)}")
+        kst, ksh, vst, vsh = ks[2], ks[1], vs[2], vs[1]
+    else:
+        T, H, d = shape
+        kst, ksh, vst, vsh = ks[0], ks[1], vs[0], vs[1]
+    if (H, d) != (ph, D):
+        raise ValueError(f"pool holds {ph} heads x {D} dims, keys are {H} x {d}")
     slots = _slots("slot_mapping", slot_mapping)
     if slots.numel() != T:
         raise ValueError(f"{T} tokens but {slots.numel()} slots")
     code = dtype_code(key.dtype)
     if T == 0:
         return
-    with _on(dev):
-        rc = L.lib().mf_q4_reshape_and_cache(
-            key.data_ptr(), value.data_ptr(), code, key.stride(0), key.stride(1), value.stride(0),
-            value.stride(1), pool.data_ptr(), pool.stride(0), pool.stride(1), pool.shape[0],
-            slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, T, H, D,
-            err_word(dev).data_ptr(), _stream_ptr(dev))
-    L.check(rc, "mf_q4_reshape_and_cache")
+    args = (key.data_ptr(), value.data_ptr(), code, kst, ksh, vst, vsh, ptr, sb, sh, nb,
+            slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, T, H, D, _err_ptr(dev),
+            _stream_ptr(dev))
+    if dev.index == torch.cuda.current_device():
+        rc = L.lib().mf_q4_reshape_and_cache(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = L.lib().mf_q4_reshape_and_cache(*args)
+    if rc:
+        L.check(rc, "mf_q4_reshape_and_cache")
     launch_counter["q4_reshape_and_cache"] += 1
-    _after("q4_reshape_and_cache", dev)
+    if _checks:
+        _after("q4_reshape_and_cache", dev)
 
 
-def q4_gather_kv(pool: torch.Tensor, flat_index: torch.Tensor,
-                 dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+def q4_gather_kv(pool: torch.Tensor, flat_index: torch.Tensor, dtype: torch.dtype, *,
+                 layer: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """
     ``mf_q4_gather_kv``: slots ``flat_index`` of one 4-bit pool layer, dequantised to
     contiguous ``(1, H, T, D)`` keys and values of ``dtype``.
     """
     dev = pool.device
     require_cuda("q4_gather_kv", pool)
-    D = q4_head_dim(pool)
+    ptr, sb, sh, nb, H, D = _q4_layer(pool, layer)
     code = dtype_code(dtype)
     if flat_index.device != dev:
         flat_index = flat_index.to(dev)
     index = _slots("flat_index", flat_index)
-    T, H = index.numel(), pool.shape[1]
+    T = index.numel()
     k = torch.empty((1, H, T, D), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     if T == 0:
         return k, v
-    with _on(dev):
-        rc = L.lib().mf_q4_gather_kv(
-            pool.data_ptr(), pool.stride(0), pool.stride(1), pool.shape[0], index.data_ptr(),
-            1 if index.dtype == torch.int64 else 0, T, H, D, k.data_ptr(), v.data_ptr(), code,
-            T * D, D, err_word(dev).data_ptr(), _stream_ptr(dev))
-    L.check(rc, "mf_q4_gather_kv")
+    args = (ptr, sb, sh, nb, index.data_ptr(), 1 if index.dtype == torch.int64 else 0, T, H, D,
+            k.data_ptr(), v.data_ptr(), code, T * D, D, _err_ptr(dev), _stream_ptr(dev))
+    if dev.index == torch.cuda.current_device():
+        rc = L.lib().mf_q4_gather_kv(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = L.lib().mf_q4_gather_kv(*args)
+    if rc:
+        L.check(rc, "mf_q4_gather_kv")
     launch_counter["q4_gather_kv"] += 1
-    _after("q4_gather_kv", dev)
+    if _checks:
+        _after("q4_gather_kv", dev)
     return k, v
+
+
+_q4_need: Dict[tuple, int] = {}   # workspace bytes by the sizes they depend on
 
 
 def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
@@ -556,28 +614,31 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
                        row_map: Optional[torch.Tensor] = None, softcap: float = 0.0,
                        window: int = 0, alibi_slopes: Optional[torch.Tensor] = None,
                        prefix_lens: Optional[torch.Tensor] = None,
-                       workspace_tensor: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       workspace_tensor: Optional[torch.Tensor] = None,
+                       layer: Optional[int] = None) -> torch.Tensor:
     """
     ``mf_q4_paged_attention`` on torch tensors: q, out ``(rows, Hq, D)`` views (any row
-    and head strides, D contiguous), one 4-bit pool layer, and tables, lengths,
-    rows and score modifiers as in :func:`paged_attention`.  The workspace is scratch
-    of the caching allocator unless one is given.
+    and head strides, D contiguous), one 4-bit pool layer (``layer``: of a pool with a
+    layer dimension), and tables, lengths, rows and score modifiers as in
+    :func:`paged_attention`.  The workspace is scratch of the caching allocator unless
+    one is given.
     """
     dev = q.device
     require_one_device("q4_paged_attention", dev, q, out, pool, block_tables, kv_lens,
                        cu_seqlens_q, row_map, workspace_tensor)
-    D = q4_head_dim(pool)
-    for name, t in (("block_tables", block_tables), ("kv_lens", kv_lens),
-                    ("cu_seqlens_q", cu_seqlens_q), ("row_map", row_map)):
-        if t is not None and t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32 (got {t.dtype})")
-    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype:
+    ptr, sb, sh, nb, hkv, D = _q4_layer(pool, layer)
+    i32 = torch.int32
+    if block_tables.dtype != i32 or kv_lens.dtype != i32 or (
+            cu_seqlens_q is not None and cu_seqlens_q.dtype != i32) or (
+            row_map is not None and row_map.dtype != i32):
+        raise TypeError("block_tables, kv_lens, cu_seqlens_q and row_map must be int32")
+    shape, qs, os_ = q.shape, q.stride(), out.stride()
+    if len(shape) != 3 or out.shape != shape or out.dtype != q.dtype:
         raise ValueError(f"q and out must be (rows, heads, D) of one shape and dtype, got "
-                         f"{tuple(q.shape)} {q.dtype} and {tuple(out.shape)} {out.dtype}")
-    if q.stride(-1) != 1 or out.stride(-1) != 1:
+                         f"{tuple(shape)} {q.dtype} and {tuple(out.shape)} {out.dtype}")
+    if qs[2] != 1 or os_[2] != 1:
         raise ValueError("q/out need a contiguous head_dim")
-    rows, hq, d = q.shape
-    hkv = pool.shape[1]
+    rows, hq, d = shape
     if d != D:
         raise ValueError(f"query head_dim {d} but the pool holds {D}")
     if hq % hkv:
@@ -588,44 +649,56 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
     if cu_seqlens_q is not None:
         if cu_seqlens_q.numel() != num_seqs + 1 or max_q_len is None:
             raise ValueError("cu_seqlens_q needs num_seqs + 1 offsets and max_q_len")
-        cu_seqlens_q = cu_seqlens_q.contiguous()
-    elif q_per_seq * num_seqs != rows:
-        raise ValueError(f"{num_seqs} sequences of {q_per_seq} rows but {rows} query rows")
-    if row_map is not None and (row_map.numel() != rows or not row_map.is_contiguous()):
-        raise ValueError("row_map must be contiguous with one entry per row")
-    if block_tables.stride(1) != 1:
+        if not cu_seqlens_q.is_contiguous():
+            cu_seqlens_q = cu_seqlens_q.contiguous()
+        most = int(max_q_len)
+    else:
+        if q_per_seq * num_seqs != rows:
+            raise ValueError(f"{num_seqs} sequences of {q_per_seq} rows but {rows} query rows")
+        most = q_per_seq
+    if row_map is not None and (row_map.numel() < rows or not row_map.is_contiguous()):
+        raise ValueError("row_map must be contiguous with an entry for each row")
+    ts = block_tables.stride()
+    if ts[1] != 1:
         block_tables = block_tables.contiguous()
-    kv_lens = kv_lens.contiguous()
-    a = L.Q4AttentionArgs()
-    a.struct_size = ctypes.sizeof(L.Q4AttentionArgs)
-    a.q, a.q_stride_row, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1)
-    a.out, a.out_stride_row, a.out_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
-    a.pool, a.pool_stride_block, a.pool_stride_head = (pool.data_ptr(), pool.stride(0),
-                                                       pool.stride(1))
-    a.num_blocks = pool.shape[0]
-    # A row of the table holds `width` entries; rows may lie further apart.
-    a.block_tables, a.table_stride = block_tables.data_ptr(), block_tables.stride(0)
-    a.table_width = block_tables.shape[1]
-    a.cu_seqlens_q, a.q_per_seq = _ptr(cu_seqlens_q), q_per_seq
-    a.kv_lens, a.row_map = kv_lens.data_ptr(), _ptr(row_map)
-    a.num_seqs, a.total_q = num_seqs, rows
-    a.max_q_len = max_q_len if max_q_len is not None else q_per_seq
-    a.num_q_heads, a.num_kv_heads, a.head_dim = hq, hkv, D
-    a.scale, a.causal, a.dtype = float(scale), 1 if causal else 0, dtype_code(q.dtype)
+        ts = block_tables.stride()
+    if not kv_lens.is_contiguous():
+        kv_lens = kv_lens.contiguous()
+    width, code = block_tables.shape[1], dtype_code(q.dtype)
+    a = L.Q4AttentionArgs(
+        ctypes.sizeof(L.Q4AttentionArgs), q.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0],
+        os_[1], ptr, sb, sh, nb, block_tables.data_ptr(), ts[0], width, _ptr(cu_seqlens_q),
+        q_per_seq, kv_lens.data_ptr(), _ptr(row_map), num_seqs, rows, most, hq, hkv, D, scale,
+        1 if causal else 0, code)
     mods = score_mods(dev, hq, num_seqs, softcap, window, alibi_slopes, prefix_lens)
     if mods is not None:
         a.mods = mods
     lib = L.lib()
-    with _on(dev):
-        need = lib.mf_q4_paged_attention_workspace_size(a, dev.index)
-        ws = workspace_tensor
-        if ws is None:
-            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        rc = lib.mf_q4_paged_attention(a, ws.data_ptr(), ws.numel() * ws.element_size(),
-                                       err_word(dev).data_ptr(), _stream_ptr(dev))
-    L.check(rc, "mf_q4_paged_attention")
+    ws, nbytes = workspace_tensor, 0
+    if ws is None:
+        key = (dev.index, code, D, hq, hkv, num_seqs, most, width, cu_seqlens_q is None,
+               mods is None, rows == 0)
+        nbytes = _q4_need.get(key)
+        if nbytes is None:
+            nbytes = lib.mf_q4_paged_attention_workspace_size(a, dev.index)
+            if len(_q4_need) > 4096:
+                _q4_need.clear()
+            _q4_need[key] = nbytes
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    else:
+        nbytes = ws.numel() * ws.element_size()
+    args = (a, _ptr(ws), nbytes, _err_ptr(dev), _stream_ptr(dev))
+    if dev.index == torch.cuda.current_device():
+        rc = lib.mf_q4_paged_attention(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = lib.mf_q4_paged_attention(*args)
+    if rc:
+        L.check(rc, "mf_q4_paged_attention")
     launch_counter["q4_paged_attention"] += 1
-    _after("q4_paged_attention", dev)
+    if _checks:
+        _after("q4_paged_attention", dev)
     return out
 
 

@@ -58,11 +58,12 @@ constexpr float PV_TOP = 128.f;     // largest sv * kinv; p <= 2^8 makes 2^15 < 
 struct Params {
   AttnParams a;  // kp: the pool, sb / sh: its block and head strides in bytes
   int G, RT;      // query heads per kv head; most row tiles of a sequence
+  uint32_t g_mul; // ceil(2^32 / G): rows are divided by G a few times per unit
   int min_tiles;  // fewest pages a CTA is given
   int rows_cap;   // runs of more rows per kv head belong to another kernel (0: none do)
   int width;      // entries of a block table's row
   int vec;        // q and out rows allow 16-byte loads and 8-byte stores
-  int64_t* prefix;   // [num_seqs + 1]
+  int32_t* prefix;   // [num_seqs + 1]
   float* part;
   int part_floats;
 };
@@ -72,6 +73,12 @@ struct Geo {
   int pfx, pa, gap, n;           // prefix keys, its pages, pages left out after them, pages
   int nrt;
 };
+
+// r / G for rows of a run (below 2^24, G at most 255: the host checks), and r % G.
+MF_DEVINL int div_g(const Params& P, int r) {
+  return P.G == 1 ? r : (int)__umulhi((uint32_t)r, P.g_mul);
+}
+MF_DEVINL int mod_g(const Params& P, int r) { return r - div_g(P, r) * P.G; }
 
 template <bool MOD>
 MF_DEVINL Geo seq_geo(const Params& P, int s, int rows, bool report) {
@@ -109,20 +116,21 @@ MF_DEVINL Geo seq_geo(const Params& P, int s, int rows, bool report) {
   return g;
 }
 
-// The tile list [0, total) cut into nv equal ranges.
+// The tile list [0, total) cut into nv equal ranges.  Tiles are counted in 32 bits (the host
+// refuses calls whose tables could hold more).
 struct Split {
-  int64_t total, nv, base, rem;
-  MF_DEVINL int64_t bound(int64_t c) const { return c >= nv ? total : c * base + min(c, rem); }
-  MF_DEVINL int owner(int64_t t) const {
-    const int64_t big = (base + 1) * rem;
+  uint32_t total, nv, base, rem;
+  MF_DEVINL uint32_t bound(uint32_t c) const { return c >= nv ? total : c * base + min(c, rem); }
+  MF_DEVINL int owner(uint32_t t) const {
+    const uint32_t big = (base + 1) * rem;
     return (int)(t < big ? t / (base + 1) : rem + (t - big) / base);
   }
 };
 
-MF_DEVINL Split make_split(int64_t total, int64_t most, int min_tiles) {
+MF_DEVINL Split make_split(uint32_t total, uint32_t most, uint32_t min_tiles) {
   Split s;
   s.total = total;
-  s.nv = min(max((total + min_tiles - 1) / min_tiles, (int64_t)1), most);
+  s.nv = min(max((total + min_tiles - 1) / min_tiles, 1u), most);
   s.base = total / s.nv;
   s.rem = total - s.base * s.nv;
   return s;
@@ -131,30 +139,30 @@ MF_DEVINL Split make_split(int64_t total, int64_t most, int min_tiles) {
 // A position in a CTA's range: the unit (s, rt, h) and the next of its pages.
 template <int R, bool MOD>
 struct Cursor {
-  int64_t pos, base;  // start of the piece after this one; first tile of sequence s
+  uint32_t pos, base;  // start of the piece after this one; first tile of sequence s
   int s, rt, h, k, k0, k1;
   Geo g;
   int hi_max, lo_min;
   bool valid;
 
-  MF_DEVINL void open(const Params& P, int64_t end) {  // the piece that starts at `pos`
+  MF_DEVINL void open(const Params& P, uint32_t end) {  // the piece that starts at `pos`
     valid = pos < end;
     if (!valid) return;
-    int64_t in = pos - base;
-    while (in >= (int64_t)g.n * g.nrt * P.a.hkv) {
-      base += (int64_t)g.n * g.nrt * P.a.hkv;
+    uint32_t in = pos - base;
+    while (in >= (uint32_t)(g.n * g.nrt * P.a.hkv)) {
+      base += (uint32_t)(g.n * g.nrt * P.a.hkv);
       g = seq_geo<MOD>(P, ++s, R, false);
       in = pos - base;
     }
-    const int64_t u = in / g.n;
+    const uint32_t u = in / (uint32_t)g.n;
     k0 = (int)(in - u * g.n);
-    rt = (int)(u / P.a.hkv);
-    h = (int)(u - (int64_t)rt * P.a.hkv);
-    k1 = (int)min((int64_t)g.n, k0 + (end - pos));
+    rt = P.RT == 1 ? 0 : (int)(u / (uint32_t)P.a.hkv);
+    h = (int)u - rt * P.a.hkv;
+    k1 = (int)min((uint32_t)g.n, k0 + (end - pos));
     pos += k1 - k0;
     const int last = min(rt * R + R, g.q_len * P.G) - 1;
-    hi_max = P.a.causal ? g.win0 + last / P.G : g.kv - 1;
-    lo_min = MOD && P.a.mods.window > 0 ? g.win0 + (rt * R) / P.G - P.a.mods.window + 1 : 0;
+    hi_max = P.a.causal ? g.win0 + div_g(P, last) : g.kv - 1;
+    lo_min = MOD && P.a.mods.window > 0 ? g.win0 + div_g(P, rt * R) - P.a.mods.window + 1 : 0;
   }
   MF_DEVINL int page(int i) const { return !MOD || i < g.pa ? i : i + g.gap; }
   MF_DEVINL bool live(int pg) const {  // some row of the tile sees some key of the page
@@ -218,13 +226,18 @@ struct Cfg {
   // CTAs per SM by registers: 32 accumulators and 16 q registers per 8 rows at D = 128.
   static constexpr int WORK = D * NT * (SPLIT ? 2 : 1);
   static constexpr int MINB = WORK <= 128 ? 4 : WORK <= 256 ? 3 : 2;
-  static constexpr int NSTG = D == 256 ? 3 : D == 128 ? 4 : 8;
-  static constexpr int BUF_LD = D + 4;  // padded row of a partial in shared memory
+  // Pages a warp takes in one step: two where the registers allow, for half the steps'
+  // fixed cost (wait, vote, copy, loop) per page and twice the independent products.
+  static constexpr int TP = NT == 1 && D <= 128 ? 2 : 1;
+  static constexpr int NSTG = D == 256 ? 3 : D == 128 ? 5 : 8;
+  static constexpr int DH = D / 2;       // dims joined in one pass through shared memory
+  static constexpr int BUF_LD = DH + 4;  // padded row of a partial there
   static constexpr int OFF_BUF = WARPS * NSTG * REC;
   static constexpr int OFF_ML = OFF_BUF + WARPS * 8 * BUF_LD * 4;
   static constexpr int OFF_BAR = OFF_ML + WARPS * R * 8;
   static constexpr int OFF_MISC = OFF_BAR + WARPS * NSTG * 8;
-  static constexpr int SMEM = OFF_MISC + 64;
+  static constexpr int OFF_CUR = OFF_MISC + 64;  // the producers' cursors, off the registers
+  static constexpr int SMEM = OFF_CUR + WARPS * 128;
 };
 
 template <typename T, int D, int NT, bool MOD>
@@ -232,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
     attn_kernel(const __grid_constant__ Params P) {
   using C = Cfg<T, D, NT>;
   using MM = Mma<__half>;
-  constexpr int R = C::R, NSTG = C::NSTG, REC = C::REC;
+  constexpr int R = C::R, NSTG = C::NSTG, REC = C::REC, TP = C::TP;
   constexpr int NW = D / 32;                   // code words per thread and row
   constexpr int VEC = NW < 4 ? NW : 4;         // of which one shared load brings VEC
   constexpr int NL = NW / VEC;
@@ -241,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
   auto hi4 = [](uint32_t w) { return operand<C::SPLIT, true>(w); };
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  int64_t* misc64 = reinterpret_cast<int64_t*>(smem + C::OFF_MISC);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, t4 = lane & 3;
   const int B = P.a.num_seqs;
@@ -256,99 +269,121 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
   // ------------------------------------------ tiles of all sequences, and my range
   const int per = (B + THREADS - 1) / THREADS;
   const int s_lo = min(tid * per, B), s_hi = min(s_lo + per, B);
-  int64_t mine = 0;
+  uint32_t mine = 0;
+  Geo first{};  // of sequence s_lo
   for (int s = s_lo; s < s_hi; ++s) {
     const Geo g = seq_geo<MOD>(P, s, R, blockIdx.x == 0);
-    mine += (int64_t)g.n * g.nrt * P.a.hkv;
+    if (s == s_lo) first = g;
+    mine += (uint32_t)(g.n * g.nrt * P.a.hkv);
   }
-  int64_t incl = mine;
+  uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) misc64[warp] = incl;
+  if (lane == 31) misc[warp] = incl;
   __syncthreads();
-  int64_t before = incl - mine, total = 0;
+  uint32_t before = incl - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += misc64[w];
-    total += misc64[w];
+    if (w < warp) before += misc[w];
+    total += misc[w];
   }
   if (blockIdx.x == 0) {
-    int64_t at = before;
+    uint32_t at = before;
     for (int s = s_lo; s < s_hi; ++s) {
-      P.prefix[s] = at;
-      const Geo g = seq_geo<MOD>(P, s, R, false);
-      at += (int64_t)g.n * g.nrt * P.a.hkv;
+      P.prefix[s] = (int)at;
+      const Geo g = s == s_lo ? first : seq_geo<MOD>(P, s, R, false);
+      at += (uint32_t)(g.n * g.nrt * P.a.hkv);
     }
-    if (tid == 0) P.prefix[B] = total;
+    if (tid == 0) P.prefix[B] = (int)total;
   }
   if (total == 0) return;
   const Split S = make_split(total, gridDim.x, P.min_tiles);
-  const int64_t lo = S.bound(blockIdx.x), hi = S.bound(blockIdx.x + 1);
+  const uint32_t lo = S.bound(blockIdx.x), hi = S.bound(blockIdx.x + 1);
   if (lo >= hi) return;
   if (lo >= before && lo < before + mine) {  // one thread: the sequence that holds tile lo
-    int64_t at = before;
+    uint32_t at = before;
     int s = s_lo;
     for (; s + 1 < s_hi; ++s) {
-      const Geo g = seq_geo<MOD>(P, s, R, false);
-      const int64_t t = (int64_t)g.n * g.nrt * P.a.hkv;
+      const Geo g = s == s_lo ? first : seq_geo<MOD>(P, s, R, false);
+      const uint32_t t = (uint32_t)(g.n * g.nrt * P.a.hkv);
       if (lo < at + t) break;
       at += t;
     }
-    misc64[4] = at;
-    misc64[5] = s;
+    misc[4] = at;
+    misc[5] = (uint32_t)s;
   }
   __syncthreads();
 
-  Cursor<R, MOD> cc, pc;  // consumer, producer
+  Cursor<R, MOD> cc;  // the consumer's; the producer's lies in shared memory
   cc.pos = lo;
-  cc.base = misc64[4];
-  cc.s = (int)misc64[5];
+  cc.base = misc[4];
+  cc.s = (int)misc[5];
   cc.g = seq_geo<MOD>(P, cc.s, R, false);
-  pc = cc;
-  pc.open(P, hi);
+  using Cur = Cursor<R, MOD>;
+  static_assert(sizeof(Cur) <= 128, "cursor slot");
+  Cur* pcs = reinterpret_cast<Cur*>(smem + C::OFF_CUR + warp * 128);
+  {
+    Cur pc = cc;
+    pc.open(P, hi);
+    pc.k = pc.k0 + TP * warp;
+    if (lane == 0) *pcs = pc;
+    __syncwarp();
+  }
   const uint32_t ring = smem_u32(smem) + warp * NSTG * REC;
   uint64_t* bar = bars + warp * NSTG;
   const uint64_t pol = l2_evict_first_policy();
   const uint8_t* pool = static_cast<const uint8_t*>(P.a.kp);
   bool dead = false;  // a wait gave up: no more copies or products, barriers only
   int issued = 0, taken = 0, pstage = 0;
-  int ids = 0, kb = -1;  // lane j: block id of page kb + j * WARPS of the producer's piece
-  if (pc.valid) pc.k = pc.k0 + warp;
+  // The producer's next records: lane j holds the address of this warp's j-th next page of
+  // its piece, and fetches it itself; todo: lanes whose page is still to be fetched.
+  const uint8_t* src = nullptr;
+  uint32_t todo = 0;
+  bool more = true;
 
-  auto issue = [&]() {
-    while (pc.valid) {
+  auto refill = [&]() {
+    Cur pc = *pcs;
+    while (todo == 0 && pc.valid) {
       if (pc.k >= pc.k1) {
         pc.open(P, hi);
-        if (!pc.valid) return;
-        pc.k = pc.k0 + warp;
-        kb = -1;
+        pc.k = pc.k0 + TP * warp;
         continue;
       }
-      const int k = pc.k;
-      pc.k += WARPS;
-      if (kb < 0 || k >= kb + 32 * WARPS) {
-        kb = k;
-        const int kk = k + lane * WARPS;
-        ids = kk < pc.k1 ? __ldg(P.a.tables + (int64_t)pc.s * P.a.table_stride + pc.page(kk)) : 0;
-        if (ids < 0 || ids >= P.a.num_blocks) {
+      const int k = pc.k + (lane / TP) * (TP * WARPS) + lane % TP;
+      bool want = k < pc.k1;
+      if (want) {
+        const int pg = pc.page(k);
+        want = pc.live(pg);
+        int id = want ? __ldg(P.a.tables + (int64_t)pc.s * P.a.table_stride + pg) : 0;
+        if (id < 0 || id >= P.a.num_blocks) {
           set_err(P.a.err, MF_ERR_BLOCK_ID);
-          ids = 0;
+          id = 0;
         }
+        src = pool + (int64_t)id * P.a.sb + (int64_t)pc.h * P.a.sh;
       }
-      if (!pc.live(pc.page(k))) continue;
-      const int id = __shfl_sync(0xffffffffu, ids, (k - kb) / WARPS);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bar[pstage], REC);
-        bulk_load(ring + pstage * REC, pool + (int64_t)id * P.a.sb + (int64_t)pc.h * P.a.sh, REC,
-                  &bar[pstage], pol);
-      }
-      pstage = pstage + 1 == NSTG ? 0 : pstage + 1;
-      ++issued;
-      return;
+      todo = __ballot_sync(0xffffffffu, want);
+      pc.k += 32 * WARPS;
     }
+    more = todo != 0;
+    __syncwarp();
+    if (lane == 0) *pcs = pc;
+    __syncwarp();
+  };
+  auto issue = [&]() {
+    if (todo == 0) {
+      if (more) refill();
+      if (todo == 0) return;
+    }
+    if (lane == __ffs(todo) - 1) {
+      mbar_arrive_expect_tx(&bar[pstage], REC);
+      bulk_load(ring + pstage * REC, src, REC, &bar[pstage], pol);
+    }
+    todo &= todo - 1;
+    pstage = pstage + 1 == NSTG ? 0 : pstage + 1;
+    ++issued;
   };
   for (int i = 0; i < NSTG; ++i) issue();
 
@@ -374,50 +409,54 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
         const int rr = cc.rt * R + nt * 8 + g4;
         have[nt] = rr < g.q_len * P.G;
         rowp[nt] = static_cast<const T*>(P.a.q) +
-                   (have[nt] ? (int64_t)map_row(P.a, g.q_start + rr / P.G) * P.a.q_sr +
-                                   (int64_t)(cc.h * P.G + rr % P.G) * P.a.q_sh
+                   (have[nt] ? (int64_t)map_row(P.a, g.q_start + div_g(P, rr)) * P.a.q_sr +
+                                   (int64_t)(cc.h * P.G + mod_g(P, rr)) * P.a.q_sh
                              : 0);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int r2 = cc.rt * R + nt * 8 + 2 * t4 + j;
-          qi[nt][j] = r2 / P.G;
+          qi[nt][j] = div_g(P, r2);
           slope[nt][j] = MOD && P.a.mods.slopes && r2 < g.q_len * P.G
-                             ? P.a.mods.slopes[cc.h * P.G + r2 % P.G] * kLog2e
+                             ? P.a.mods.slopes[cc.h * P.G + mod_g(P, r2)] * kLog2e
                              : 0.f;
         }
       }
-      auto load8q = [&](int nt, int i, float* x) {
-        const int dim = (i / VEC) * 128 + t4 * (8 * VEC) + (i % VEC) * 8;
-        const T* p = rowp[nt] + dim;
-        if (!have[nt]) {
+      constexpr int QV = sizeof(T) / 2;  // 16-byte loads for eight elements
+      uint4 raw[NT][NW][QV];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        } else if (P.vec) {
-          uint4 r[sizeof(T) / 2];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < (int)sizeof(T) / 2; ++e)
-            r[e] = __ldg(reinterpret_cast<const uint4*>(p) + e);
-          const T* v = reinterpret_cast<const T*>(r);
+        for (int i = 0; i < NW; ++i) {
+          const int dim = (i / VEC) * 128 + t4 * (8 * VEC) + (i % VEC) * 8;
+          const T* p = rowp[nt] + dim;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = Elt<T>::to_f32(v[e]);
-        } else {
+          for (int e = 0; e < QV; ++e) raw[nt][i][e] = make_uint4(0, 0, 0, 0);
+          if (have[nt]) {
+            if (P.vec) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = Elt<T>::to_f32(p[e]);
+              for (int e = 0; e < QV; ++e)
+                raw[nt][i][e] = __ldg(reinterpret_cast<const uint4*>(p) + e);
+            } else {
+              T v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = p[e];
+#pragma unroll
+              for (int e = 0; e < QV; ++e) raw[nt][i][e] = reinterpret_cast<const uint4*>(v)[e];
+            }
+          }
         }
-      };
       float top = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-          float x[8];
-          load8q(nt, i, x);
+          const T* v = reinterpret_cast<const T*>(raw[nt][i]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            sum += x[e];
-            const float v = fabsf(x[e]);
-            if (v <= 3.402823466e38f) top = fmaxf(top, v);  // a NaN or infinity spoils its row only
+            const float x = Elt<T>::to_f32(v[e]);
+            sum += x;
+            if (fabsf(x) <= 3.402823466e38f) top = fmaxf(top, fabsf(x));  // else its row only
           }
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -435,10 +474,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
+          const T* v = reinterpret_cast<const T*>(raw[nt][i]);
           float x[8];
-          load8q(nt, i, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= (e & 1) ? mul * 0.0625f : mul;
+          for (int e = 0; e < 8; ++e) x[e] = Elt<T>::to_f32(v[e]) * ((e & 1) ? mul * 0.0625f : mul);
 #pragma unroll
           for (int sp = 0; sp < SP; ++sp) {
 #pragma unroll
@@ -455,133 +494,197 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
         }
     }
     float o[NT][D / 16][4], ones[NT][4];
-    float m[NT][2], l[NT][2], ob[NT][2], kinv = 0.f;
+    // mu: what scores are taken relative to (0 before any key is seen); up: how far one may
+    // pass it (anything does, before).  sv_top: the largest scale that kinv serves.
+    float up[NT][2], mu[NT][2], l[NT][2], ob[NT][2], kinv = 0.f, sv_top = -1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) o[nt][n][0] = o[nt][n][1] = o[nt][n][2] = o[nt][n][3] = 0.f;
       ones[nt][0] = ones[nt][1] = ones[nt][2] = ones[nt][3] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
+      up[nt][0] = up[nt][1] = -INFINITY;
+      mu[nt][0] = mu[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = ob[nt][0] = ob[nt][1] = 0.f;
     }
     // Largest key every row sees from below, smallest every row sees from above.
-    const int first_qi = (cc.rt * R) / P.G;
+    const int first_qi = div_g(P, cc.rt * R);
     const int hi_all = P.a.causal ? min(g.win0 + first_qi, g.kv - 1) : g.kv - 1;
-    const int last_qi = (min(cc.rt * R + R, g.q_len * P.G) - 1) / P.G;
+    const int last_qi = div_g(P, min(cc.rt * R + R, g.q_len * P.G) - 1);
     const int lo_all = MOD && P.a.mods.window > 0 ? g.win0 + last_qi - P.a.mods.window + 1 : 0;
 
-    for (int k = cc.k0 + warp; k < cc.k1; k += WARPS) {
-      const int pg = cc.page(k);
-      if (!cc.live(pg)) continue;
-      if (!dead && !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT)) dead = true;
-      dead = __any_sync(0xffffffffu, dead);
+    for (int k = cc.k0 + TP * warp; k < cc.k1; k += TP * WARPS) {
+      // The step's pages, live ones first; without a second one, its place re-reads the
+      // first record as keys that no row sees.
+      int kb[TP];
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        kb[u] = 0x7fffff00;
+        const int pg = cc.page(k + u);
+        if (k + u < cc.k1 && cc.live(pg)) {
+          if (TP == 2 && n == 0) kb[0] = pg * PAGE;
+          else kb[u] = pg * PAGE;
+          ++n;
+        }
+      }
+      if (n == 0) continue;
+      uint32_t rec[TP];
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        rec[u] = u < n ? ring + stage * REC : rec[0];
+        if (u < n) {
+          if (!__all_sync(0xffffffffu, mbar_try_wait(&bar[stage], phase))) {
+            if (!dead && !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT)) dead = true;
+            dead = __any_sync(0xffffffffu, dead);
+          }
+          if (!dead) {
+            ++taken;
+            if (++stage == NSTG) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+      }
       if (dead) continue;
-      ++taken;
-      const uint32_t rec = ring + stage * REC;
-      const int kbase = pg * PAGE;
 
       // ---------------------------------------------------------- S^T = K Q^T
       // At NT = 1 two accumulators halve the dependent chain.
-      float sc[NT][4], sd[4] = {0.f, 0.f, 0.f, 0.f};
+      float sc[TP][NT][4], sd[TP][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NL; ++c) {
-        uint32_t ka[VEC], kc[VEC];
-        lds_words<VEC>(rec + g4 * (D / 2) + c * 64 + t4 * (4 * VEC), ka);
-        lds_words<VEC>(rec + (g4 + 8) * (D / 2) + c * 64 + t4 * (4 * VEC), kc);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const uint32_t a0[4] = {lo4(ka[i]), lo4(kc[i]), hi4(ka[i]), hi4(kc[i])};
-          const uint32_t ka8 = ka[i] >> 8, kc8 = kc[i] >> 8;
-          const uint32_t a1[4] = {lo4(ka8), lo4(kc8), hi4(ka8), hi4(kc8)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int sp = 0; sp < SP; ++sp) {
-              const uint32_t* q = qb[nt][sp][c * VEC + i];
-              MM::run(sc[nt], a0, q[0], q[1]);
-              MM::run(NT == 1 ? sd : sc[nt], a1, q[2], q[3]);
-            }
-        }
-      }
-      // ------------------------------------------------- scores in log2 units
-      float2 pk0 = lds_half2(rec + 16 * D + g4 * 4), pk1 = lds_half2(rec + 16 * D + 32 + g4 * 4);
-      float2 pv0 = lds_half2(rec + 16 * D + 64 + g4 * 4),
-             pv1 = lds_half2(rec + 16 * D + 96 + g4 * 4);
-      const bool need_mask =
-          kbase + PAGE - 1 > hi_all || (MOD && kbase < lo_all && kbase + PAGE > g.pfx);
-      if (kbase + PAGE > g.kv) {  // slots behind the last token hold anything
-        if (kbase + g4 >= g.kv) pk0 = pv0 = make_float2(0.f, 0.f);
-        if (kbase + g4 + 8 >= g.kv) pk1 = pv1 = make_float2(0.f, 0.f);
-      }
-      if (C::SPLIT) {  // codes were taken as n - 8
-        pk0.y = fmaf(8.f, pk0.x, pk0.y);
-        pk1.y = fmaf(8.f, pk1.x, pk1.y);
-      }
-      const float sk0 = pk0.x * cq, sk1 = pk1.x * cq;
-      uint32_t vis = 0xffffffffu;  // bit nt * 4 + e
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < TP; ++u) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int j = e & 1;
-          float s = fmaf(NT == 1 ? sc[nt][e] + sd[e] : sc[nt][e], e < 2 ? sk0 : sk1,
-                         (e < 2 ? pk0.y : pk1.y) * qs[nt][j]);
-          if (MOD) {
-            const int back = g.win0 + qi[nt][j] - (kbase + g4 + (e < 2 ? 0 : 8));
-            if (P.a.mods.softcap > 0.f) s = softcap_log2(s, cap2, two_over);
-            if (P.a.mods.slopes) s = fmaf(-slope[nt][j], (float)back, s);
-          }
-          sc[nt][e] = s;
+          sd[u][e] = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[u][nt][e] = 0.f;
         }
-      if (need_mask) {
-        vis = 0;
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+          uint32_t ka[VEC], kc[VEC];
+          lds_words<VEC>(rec[u] + g4 * (D / 2) + c * 64 + t4 * (4 * VEC), ka);
+          lds_words<VEC>(rec[u] + (g4 + 8) * (D / 2) + c * 64 + t4 * (4 * VEC), kc);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const uint32_t a0[4] = {lo4(ka[i]), lo4(kc[i]), hi4(ka[i]), hi4(kc[i])};
+            const uint32_t ka8 = ka[i] >> 8, kc8 = kc[i] >> 8;
+            const uint32_t a1[4] = {lo4(ka8), lo4(kc8), hi4(ka8), hi4(kc8)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int sp = 0; sp < SP; ++sp) {
+                const uint32_t* q = qb[nt][sp][c * VEC + i];
+                MM::run(sc[u][nt], a0, q[0], q[1]);
+                MM::run(NT == 1 ? sd[u] : sc[u][nt], a1, q[2], q[3]);
+              }
+          }
+        }
+      }
+      // ------------------------------------------------- scores in log2 units, less mu
+      float sv[TP][2], bv[TP][2];  // V scale and base (of centred codes) of keys g4, g4 + 8
+      bool need_mask = false;
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        const uint32_t par = rec[u] + 16 * D + g4 * 4;
+        float2 pk0 = lds_half2(par), pk1 = lds_half2(par + 32);
+        float2 pv0 = lds_half2(par + 64), pv1 = lds_half2(par + 96);
+        need_mask = need_mask || kb[u] + PAGE - 1 > hi_all ||
+                    (MOD && kb[u] < lo_all && kb[u] + PAGE > g.pfx);
+        if (kb[u] + PAGE > g.kv) {  // slots behind the last token hold anything
+          if (kb[u] + g4 >= g.kv) pk0 = pv0 = make_float2(0.f, 0.f);
+          if (kb[u] + g4 + 8 >= g.kv) pk1 = pv1 = make_float2(0.f, 0.f);
+        }
+        if (C::SPLIT) {  // codes were taken as n - 8
+          pk0.y = fmaf(8.f, pk0.x, pk0.y);
+          pk1.y = fmaf(8.f, pk1.x, pk1.y);
+        }
+        sv[u][0] = pv0.x;
+        sv[u][1] = pv1.x;
+        bv[u][0] = C::CENTRE || C::SPLIT ? fmaf(8.f, pv0.x, pv0.y) : pv0.y;
+        bv[u][1] = C::CENTRE || C::SPLIT ? fmaf(8.f, pv1.x, pv1.y) : pv1.y;
+        const float sk0 = pk0.x * cq, sk1 = pk1.x * cq;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = kbase + g4 + (e < 2 ? 0 : 8);
-            const int qpos = g.win0 + qi[nt][e & 1];
-            bool see = !P.a.causal || key <= qpos;
-            if (MOD && P.a.mods.window > 0) see = see && qpos - key < P.a.mods.window;
-            if (MOD) see = see || key < g.pfx;
-            see = see && key < g.kv;
-            if (see) vis |= 1u << (nt * 4 + e);
-            else sc[nt][e] = -INFINITY;
+            const int j = e & 1;
+            const float raw = NT == 1 ? sc[u][nt][e] + sd[u][e] : sc[u][nt][e];
+            const float by = e < 2 ? pk0.y : pk1.y, sk = e < 2 ? sk0 : sk1;
+            float x;
+            if (MOD) {
+              const int back = g.win0 + qi[nt][j] - (kb[u] + g4 + (e < 2 ? 0 : 8));
+              x = fmaf(raw, sk, by * qs[nt][j]);
+              if (P.a.mods.softcap > 0.f) x = softcap_log2(x, cap2, two_over);
+              if (P.a.mods.slopes) x = fmaf(-slope[nt][j], (float)back, x);
+              x -= mu[nt][j];
+            } else {
+              x = fmaf(raw, sk, fmaf(by, qs[nt][j], -mu[nt][j]));
+            }
+            sc[u][nt][e] = x;
           }
       }
-      // ------------------------------------------------ running maximum, lazily
-      bool raise = fmaxf(pv0.x, pv1.x) * kinv > PV_TOP || kinv == 0.f;
+      uint32_t vis = 0xffffffffu;  // bit (u * NT + nt) * 4 + e
+      if (need_mask) {
+        vis = 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        raise = raise || fmaxf(sc[nt][0], sc[nt][2]) > m[nt][0] + RAISE;
-        raise = raise || fmaxf(sc[nt][1], sc[nt][3]) > m[nt][1] + RAISE;
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = kb[u] + g4 + (e < 2 ? 0 : 8);
+              const int qpos = g.win0 + qi[nt][e & 1];
+              bool see = !P.a.causal || key <= qpos;
+              if (MOD && P.a.mods.window > 0) see = see && qpos - key < P.a.mods.window;
+              if (MOD) see = see || key < g.pfx;
+              see = see && key < g.kv;
+              if (see) vis |= 1u << ((u * NT + nt) * 4 + e);
+              else sc[u][nt][e] = -INFINITY;
+            }
       }
+      // ------------------------------------------------ running maximum, lazily
+      float tm[NT][2], st = fmaxf(sv[0][0], sv[0][1]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          tm[nt][j] = fmaxf(sc[0][nt][j], sc[0][nt][2 + j]);
+          if (TP == 2) tm[nt][j] = fmax3f(tm[nt][j], sc[TP - 1][nt][j], sc[TP - 1][nt][2 + j]);
+        }
+      if (TP == 2) st = fmax3f(st, sv[TP - 1][0], sv[TP - 1][1]);
+      bool raise = st > sv_top;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) raise = raise || tm[nt][0] > up[nt][0] || tm[nt][1] > up[nt][1];
       if (__any_sync(0xffffffffu, raise)) {
-        float st = fmaxf(pv0.x, pv1.x);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) st = fmaxf(st, __shfl_xor_sync(0xffffffffu, st, x));
         if (!(st <= 65504.f)) st = 0.f;  // a NaN or infinite scale is no size to go by
         float fv = 1.f;
-        if (st * kinv > PV_TOP || kinv == 0.f) {
+        if (st > sv_top) {
           // 2^6 / 2^floor(log2 st): sv * kinv <= 2^7, with room for the last factor of two
           const int ex = (int)((__float_as_uint(st) >> 23) & 255u);
           const float next = __uint_as_float((uint32_t)min(max(260 - ex, 97), 160) << 23);
           fv = kinv == 0.f ? 0.f : next / kinv;
           kinv = next;
+          sv_top = PV_TOP / next;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float t = fmaxf(sc[nt][j], sc[nt][2 + j]);
+            float t = tm[nt][j];
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
             float al = 1.f;
-            if (t > m[nt][j] + RAISE) {
-              al = m[nt][j] == -INFINITY ? 0.f : fast_exp2(m[nt][j] - t);
-              m[nt][j] = t;
+            if (t > up[nt][j]) {  // t is relative to mu
+              al = up[nt][j] == -INFINITY ? 0.f : fast_exp2(-t);
+              mu[nt][j] += t;
+              up[nt][j] = RAISE;
+#pragma unroll
+              for (int u = 0; u < TP; ++u) {
+                sc[u][nt][j] -= t;
+                sc[u][nt][2 + j] -= t;
+              }
             }
             l[nt][j] *= al;
             ob[nt][j] *= al;
@@ -595,65 +698,68 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
           }
       }
       // -------------------------------------------------------------- P and sums
-      const float sv0 = pv0.x * kinv, sv1 = pv1.x * kinv;
-      const float bv0 = C::CENTRE || C::SPLIT ? fmaf(8.f, pv0.x, pv0.y) : pv0.y;
-      const float bv1 = C::CENTRE || C::SPLIT ? fmaf(8.f, pv1.x, pv1.y) : pv1.y;
-      uint32_t pb[NT][SP][2];
+      uint32_t pb[TP][NT][SP][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float pp[4];
+      for (int u = 0; u < TP; ++u) {
+        const float sv0 = sv[u][0] * kinv, sv1 = sv[u][1] * kinv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = e & 1;
-          const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-          const float p = fast_exp2(sc[nt][e] - mu);
-          l[nt][j] += p;
-          const bool see = (vis >> (nt * 4 + e)) & 1u;  // p = 0 must not meet a NaN it does not see
-          ob[nt][j] += see ? p * (e < 2 ? bv0 : bv1) : 0.f;
-          pp[e] = see ? p * (e < 2 ? sv0 : sv1) : 0.f;
-        }
+        for (int nt = 0; nt < NT; ++nt) {
+          float pp[4], pq[4];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const uint32_t w = MM::pack(pp[2 * hf], pp[2 * hf + 1]);
-          pb[nt][0][hf] = movm_trans(w);
-          if (SP == 2) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-            pb[nt][SP - 1][hf] =
-                movm_trans(MM::pack(pp[2 * hf] - f.x, pp[2 * hf + 1] - f.y));
+          for (int e = 0; e < 4; ++e) {
+            const float p = fast_exp2(sc[u][nt][e]);
+            l[nt][e & 1] += p;
+            pq[e] = p * bv[u][e >> 1];
+            pp[e] = p * (e < 2 ? sv0 : sv1);
           }
-        }
-        if (C::CENTRE) {
-          const uint32_t one[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-          MM::run(ones[nt], one, pb[nt][0][0], pb[nt][0][1]);
+          if (need_mask) {  // p = 0 must not meet a NaN that its row does not see
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!((vis >> ((u * NT + nt) * 4 + e)) & 1u)) pp[e] = pq[e] = 0.f;
+          }
+          ob[nt][0] += pq[0] + pq[2];
+          ob[nt][1] += pq[1] + pq[3];
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t w = MM::pack(pp[2 * hf], pp[2 * hf + 1]);
+            pb[u][nt][0][hf] = movm_trans(w);
+            if (SP == 2) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+              pb[u][nt][SP - 1][hf] =
+                  movm_trans(MM::pack(pp[2 * hf] - f.x, pp[2 * hf + 1] - f.y));
+            }
+          }
+          if (C::CENTRE) {
+            const uint32_t one[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+            MM::run(ones[nt], one, pb[u][nt][0][0], pb[u][nt][0][1]);
+          }
         }
       }
       // ------------------------------------------------------- O^T += V^T P^T
 #pragma unroll
-      for (int c = 0; c < NL; ++c) {
-        uint32_t va[VEC], vb[VEC];
-        const uint32_t at = rec + 8 * D + c * 1024 + lane * (4 * VEC);
-        lds_words<VEC>(at, va);
-        lds_words<VEC>(at + 128 * VEC, vb);
+      for (int u = 0; u < TP; ++u)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const uint32_t a0[4] = {lo4(va[i]), hi4(va[i]), lo4(vb[i]), hi4(vb[i])};
-          const uint32_t va8 = va[i] >> 8, vb8 = vb[i] >> 8;
-          const uint32_t a1[4] = {lo4(va8), hi4(va8), lo4(vb8), hi4(vb8)};
+        for (int c = 0; c < NL; ++c) {
+          uint32_t va[VEC], vb[VEC];
+          const uint32_t at = rec[u] + 8 * D + c * 1024 + lane * (4 * VEC);
+          lds_words<VEC>(at, va);
+          lds_words<VEC>(at + 128 * VEC, vb);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int i = 0; i < VEC; ++i) {
+            const uint32_t a0[4] = {lo4(va[i]), hi4(va[i]), lo4(vb[i]), hi4(vb[i])};
+            const uint32_t va8 = va[i] >> 8, vb8 = vb[i] >> 8;
+            const uint32_t a1[4] = {lo4(va8), hi4(va8), lo4(vb8), hi4(vb8)};
 #pragma unroll
-            for (int sp = 0; sp < SP; ++sp) {
-              MM::run(o[nt][2 * (c * VEC + i)], a0, pb[nt][sp][0], pb[nt][sp][1]);
-              MM::run(o[nt][2 * (c * VEC + i) + 1], a1, pb[nt][sp][0], pb[nt][sp][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int sp = 0; sp < SP; ++sp) {
+                MM::run(o[nt][2 * (c * VEC + i)], a0, pb[u][nt][sp][0], pb[u][nt][sp][1]);
+                MM::run(o[nt][2 * (c * VEC + i) + 1], a1, pb[u][nt][sp][0], pb[u][nt][sp][1]);
+              }
+          }
         }
-      }
       __syncwarp();
-      if (++stage == NSTG) {
-        stage = 0;
-        phase ^= 1u;
-      }
-      issue();
+      for (int u = 0; u < n; ++u) issue();
     }
 
     // --------------------------------------------------- join the four warps' parts
@@ -668,76 +774,92 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
           l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], x);
           ob[nt][j] += __shfl_xor_sync(0xffffffffu, ob[nt][j], x);
         }
-        if (g4 == 0) ml[warp * R + nt * 8 + 2 * t4 + j] = make_float2(m[nt][j], l[nt][j]);
+        if (up[nt][j] == -INFINITY) mu[nt][j] = -INFINITY;  // no key was seen
+        if (g4 == 0) ml[warp * R + nt * 8 + 2 * t4 + j] = make_float2(mu[nt][j], l[nt][j]);
       }
+    __syncthreads();
+    // One warp: each row's common maximum M and sum L, every warp's factor to M.
+    for (int row = tid; row < R; row += THREADS) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, ml[w * R + row].x);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float2 v = ml[w * R + row];
+        const float f = v.x == -INFINITY ? 0.f : fast_exp2(v.x - M);
+        L += v.x == -INFINITY ? v.y : v.y * f;  // (a row of NaN scores has no maximum)
+        ml[w * R + row].x = f;
+      }
+      if (whole) {
+        ml[row].y = L == 0.f ? 0.f : 1.f / L;
+      } else {
+        slot[R * D + row] = M;
+        slot[R * D + R + row] = L;
+      }
+    }
     __syncthreads();
     const float inv_k = kinv > 0.f ? 1.f / kinv : 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = 2 * t4 + j;
-        float M = -INFINITY;
+      for (int half = 0; half < 2; ++half) {  // words [half * NW / 2, + NW / 2) of each thread
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, ml[w * R + nt * 8 + row].x);
-        const float f = m[nt][j] == -INFINITY ? 0.f : fast_exp2(m[nt][j] - M);
-        const float add = f * (ob[nt][j] - (C::CENTRE ? 8.f * ones[nt][j] * inv_k : 0.f));
-        const float fo = f * C::UNIT * inv_k, fo16 = fo * 0.0625f;
-        float* dst = buf + (warp * 8 + row) * C::BUF_LD;
+        for (int j = 0; j < 2; ++j) {
+          const int row = 2 * t4 + j;
+          const float f = ml[warp * R + nt * 8 + row].x;
+          const float add = f * (ob[nt][j] - (C::CENTRE ? 8.f * ones[nt][j] * inv_k : 0.f));
+          const float fo = f * C::UNIT * inv_k, fo16 = fo * 0.0625f;
+          float* dst = buf + (warp * 8 + row) * C::BUF_LD + g4 * (NW * 2);
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-          const int dim = (i / VEC) * 128 + g4 * (4 * VEC) + (i % VEC) * 4;
-          const float* x0 = o[nt][2 * i];
-          const float* x1 = o[nt][2 * i + 1];
-          *reinterpret_cast<float4*>(dst + dim) =
-              make_float4(fmaf(x0[j], fo, add), fmaf(x0[2 + j], fo16, add), fmaf(x1[j], fo, add),
-                          fmaf(x1[2 + j], fo16, add));
+          for (int i = 0; i < NW / 2; ++i) {
+            const float* x0 = o[nt][2 * (half * (NW / 2) + i)];
+            const float* x1 = o[nt][2 * (half * (NW / 2) + i) + 1];
+            *reinterpret_cast<float4*>(dst + i * 4) =
+                make_float4(fmaf(x0[j], fo, add), fmaf(x0[2 + j], fo16, add),
+                            fmaf(x1[j], fo, add), fmaf(x1[2 + j], fo16, add));
+          }
         }
-      }
-      __syncthreads();
-      for (int idx = tid; idx < 8 * (D / 4); idx += THREADS) {
-        const int row = idx / (D / 4), col = (idx % (D / 4)) * 4;
-        const int rr = cc.rt * R + nt * 8 + row;
-        if (rr >= g.q_len * P.G) continue;
-        float M = -INFINITY, L = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+        for (int idx = tid; idx < 8 * (C::DH / 4); idx += THREADS) {
+          const int row = idx / (C::DH / 4), in = idx % (C::DH / 4);
+          // thread group in / (NW / 2), its word half * NW / 2 + in % (NW / 2)
+          const int wd = half * (NW / 2) + in % (NW / 2);
+          const int col = (wd / VEC) * 128 + (in / (NW / 2)) * (4 * VEC) + (wd % VEC) * 4;
+          const int rr = cc.rt * R + nt * 8 + row;
+          if (rr >= g.q_len * P.G) continue;
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, ml[w * R + nt * 8 + row].x);
+          for (int w = 0; w < WARPS; ++w) {
+            const float4 b =
+                *reinterpret_cast<const float4*>(buf + (w * 8 + row) * C::BUF_LD + in * 4);
+            a.x += b.x;
+            a.y += b.y;
+            a.z += b.z;
+            a.w += b.w;
+          }
+          if (whole) {
+            const float inv = ml[nt * 8 + row].y;
+            T* dst = static_cast<T*>(P.a.out) +
+                     (int64_t)map_row(P.a, g.q_start + div_g(P, rr)) * P.a.o_sr +
+                     (int64_t)(cc.h * P.G + mod_g(P, rr)) * P.a.o_sh + col;
+            T e[4] = {from_f32<T>(a.x * inv), from_f32<T>(a.y * inv), from_f32<T>(a.z * inv),
+                      from_f32<T>(a.w * inv)};
+            if (P.vec) {
+              if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(e);
+              else
+                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(e);
+            } else {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          const float2 v = ml[w * R + nt * 8 + row];
-          L += v.x == -INFINITY ? v.y : v.y * fast_exp2(v.x - M);
-          const float4 b = *reinterpret_cast<const float4*>(buf + (w * 8 + row) * C::BUF_LD + col);
-          a.x += b.x;
-          a.y += b.y;
-          a.z += b.z;
-          a.w += b.w;
-        }
-        if (whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          T* dst = static_cast<T*>(P.a.out) +
-                   (int64_t)map_row(P.a, g.q_start + rr / P.G) * P.a.o_sr +
-                   (int64_t)(cc.h * P.G + rr % P.G) * P.a.o_sh + col;
-          T e[4] = {from_f32<T>(a.x * inv), from_f32<T>(a.y * inv), from_f32<T>(a.z * inv),
-                    from_f32<T>(a.w * inv)};
-          if (P.vec) {
-            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(e);
-            else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(e);
+              for (int i = 0; i < 4; ++i) dst[i] = e[i];
+            }
           } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dst[i] = e[i];
-          }
-        } else {
-          const int pr = nt * 8 + row;
-          *reinterpret_cast<float4*>(slot + pr * D + col) = a;
-          if (col == 0) {
-            slot[R * D + pr] = M;
-            slot[R * D + R + pr] = L;
+            const int pr = nt * 8 + row;
+            *reinterpret_cast<float4*>(slot + pr * D + col) = a;
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
-    }
   }
   if (dead) {  // copies in flight still target this CTA's shared memory
     if (lane == 0) set_err(P.a.err, MF_ERR_TIMEOUT);
@@ -765,8 +887,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
   int c0 = 0, c1 = 0;
   Split S;
   if (g.n > 0) {
-    S = make_split(P.prefix[P.a.num_seqs], ranges, P.min_tiles);
-    const int64_t start = P.prefix[s] + (int64_t)u * g.n;
+    S = make_split((uint32_t)P.prefix[P.a.num_seqs], ranges, P.min_tiles);
+    const uint32_t start = (uint32_t)P.prefix[s] + (uint32_t)u * g.n;
     c0 = S.owner(start);
     c1 = S.owner(start + g.n - 1);
     if (c0 == c1) return;  // written whole
@@ -798,8 +920,9 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    T* dst = static_cast<T*>(P.a.out) + (int64_t)map_row(P.a, g.q_start + rr / P.G) * P.a.o_sr +
-             (int64_t)(h * P.G + rr % P.G) * P.a.o_sh + col;
+    T* dst = static_cast<T*>(P.a.out) +
+             (int64_t)map_row(P.a, g.q_start + div_g(P, rr)) * P.a.o_sr +
+             (int64_t)(h * P.G + mod_g(P, rr)) * P.a.o_sh + col;
     dst[0] = from_f32<T>(a.x * inv);
     dst[1] = from_f32<T>(a.y * inv);
     dst[2] = from_f32<T>(a.z * inv);
@@ -919,6 +1042,10 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
   P.a.err = err;
   P.a.mods = {a->mods.softcap, a->mods.alibi_slopes, a->mods.window, a->mods.prefix_lens};
   P.G = a->num_q_heads / a->num_kv_heads;
+  P.g_mul = (uint32_t)(((1ull << 32) + P.G - 1) / P.G);
+  if (P.G > 255 || (int64_t)P.a.max_q_len * P.G >= (1 << 24))
+    return fail(MF_EUNSUPPORTED, "q4 attention: more than 255 query heads per kv head, or 2^24 "
+                                 "rows of a run");
   const int64_t es = a->dtype == MF_F32 ? 4 : 2;
   P.vec = (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15) == 0 &&
            (a->q_stride_row * es) % 16 == 0 && (a->q_stride_head * es) % 16 == 0 &&
@@ -950,7 +1077,7 @@ Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
   pl.ranges = (int)std::min<int64_t>((int64_t)sms * per_sm,
                                      std::max<int64_t>((most + P.min_tiles - 1) / P.min_tiles, 1));
   pl.part_floats = 8 * pl.nt * (P.a.d + 2);
-  pl.prefix_bytes = ((size_t)(P.a.num_seqs + 1) * 8 + 255) & ~(size_t)255;
+  pl.prefix_bytes = ((size_t)(P.a.num_seqs + 1) * 4 + 255) & ~(size_t)255;
   pl.ws_bytes = pl.prefix_bytes + (size_t)pl.ranges * 2 * pl.part_floats * sizeof(float);
   return pl;
 }
@@ -979,12 +1106,14 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
   if (P.a.num_seqs == 0 || P.a.total_q == 0 || P.a.max_q_len == 0) return MF_OK;
   const Plan pl = make_plan(P, args->dtype, current_sm_count());
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (pl.rt * P.a.hkv > 0x7fffffffLL) return fail(MF_EUNSUPPORTED, "q4 attention: too many row tiles");
+  if (pl.tiles && (double)pl.rt * P.a.hkv * P.a.num_seqs * P.width >= 2147483648.0)
+    return fail(MF_EUNSUPPORTED, "q4 attention: the tables could hold 2^31 or more (row tile, "
+                                 "page) pairs");
   if (pl.tiles && (!workspace || workspace_bytes < pl.ws_bytes ||
                    (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail(MF_EWORKSPACE, "q4 attention: workspace missing, misaligned or smaller than "
                                "mf_q4_paged_attention_workspace_size()");
-  P.prefix = static_cast<int64_t*>(workspace);
+  P.prefix = static_cast<int32_t*>(workspace);
   if (pl.tiles) P.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.prefix_bytes);
   P.part_floats = pl.part_floats;
   if (pl.chunks) {

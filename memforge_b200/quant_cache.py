@@ -42,11 +42,7 @@ def scatter_kv_q4(pool: torch.Tensor, layer_idx: int, flat_index: torch.Tensor,
     ``flat_index`` (-1 skips a token), in place: ``paged_gather.scatter_kv`` for a
     4-bit pool.  Sources are fp32, fp16 or bf16, of any strides.
     """
-    if keys.dim() != 4 or keys.shape[0] != 1 or values.dim() != 4 or values.shape[0] != 1:
-        raise ValueError(f"keys/values must be (1, heads, tokens, head_dim), got "
-                         f"{tuple(keys.shape)} and {tuple(values.shape)}")
-    K.q4_reshape_and_cache(keys[0].transpose(0, 1), values[0].transpose(0, 1), pool[layer_idx],
-                           flat_index)
+    K.q4_reshape_and_cache(keys, values, pool, flat_index, layer=layer_idx, heads_first=True)
 
 
 def gather_kv_q4(pool: torch.Tensor, layer_idx: int, flat_index: torch.Tensor,
@@ -55,7 +51,7 @@ def gather_kv_q4(pool: torch.Tensor, layer_idx: int, flat_index: torch.Tensor,
     The slots ``flat_index`` of a layer as dequantised ``(1, heads, tokens,
     head_dim)`` K/V of ``dtype``: ``paged_gather.gather_kv`` for a 4-bit pool.
     """
-    return K.q4_gather_kv(pool[layer_idx], flat_index, dtype)
+    return K.q4_gather_kv(pool, flat_index, dtype, layer=layer_idx)
 
 
 def paged_attention_q4(q: torch.Tensor, pool: torch.Tensor, layer_idx: int,
@@ -80,10 +76,10 @@ def paged_attention_q4(q: torch.Tensor, pool: torch.Tensor, layer_idx: int,
     if q.stride(-1) != 1:
         q = q.contiguous()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    return K.q4_paged_attention(q, out, pool[layer_idx], block_tables, kv_lens,
+    return K.q4_paged_attention(q, out, pool, block_tables, kv_lens, layer=layer_idx,
                                 cu_seqlens_q=cu_seqlens_q, q_per_seq=q_per_seq,
                                 max_q_len=max_q_len, scale=scale, causal=causal, row_map=row_map,
                                 softcap=softcap, window=window, alibi_slopes=alibi_slopes,
@@ -133,11 +129,12 @@ class Q4KVPool(PagedKVPool):
 
     def write_rows(self, layer_idx: int, keys: torch.Tensor, values: torch.Tensor,
                    slots: torch.Tensor) -> None:
-        K.q4_reshape_and_cache(keys, values, self.pool[layer_idx], slots)
+        K.q4_reshape_and_cache(keys, values, self.pool, slots, layer=layer_idx)
 
     def attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor,
                block_tables: torch.Tensor, kv_lens: torch.Tensor, **how) -> torch.Tensor:
-        return K.q4_paged_attention(q, out, self.pool[layer_idx], block_tables, kv_lens, **how)
+        return K.q4_paged_attention(q, out, self.pool, block_tables, kv_lens, layer=layer_idx,
+                                    **how)
 
     def zero_(self) -> None:
         self.pool.zero_()

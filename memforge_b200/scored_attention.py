@@ -54,7 +54,7 @@ def paged_attention_scored(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
     if q.stride(-1) != 1:
         q = q.contiguous()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return K.paged_attention(q, out, key_pool[layer_idx], value_pool[layer_idx], block_tables,
