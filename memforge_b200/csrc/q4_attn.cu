@@ -372,20 +372,30 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
     if (lane == 0) *pcs = pc;
     __syncwarp();
   };
-  auto issue = [&]() {
-    if (todo == 0) {
-      if (more) refill();
-      if (todo == 0) return;
+  // Fetches the next `want` (1 or 2) records, each by the lane that holds its address.
+  auto issue = [&](int want) {
+    while (want > 0) {
+      if (todo == 0) {
+        if (more) refill();
+        if (todo == 0) return;
+      }
+      const uint32_t rest = todo & (todo - 1);
+      const int l0 = __ffs(todo) - 1, l1 = want == 2 && rest ? __ffs(rest) - 1 : l0;
+      const int next = pstage + 1 == NSTG ? 0 : pstage + 1;
+      if (lane == l0 || lane == l1) {
+        const int st = lane == l0 ? pstage : next;
+        mbar_arrive_expect_tx(&bar[st], REC);
+        bulk_load(ring + st * REC, src, REC, &bar[st], pol);
+      }
+      const bool two = l1 != l0;
+      todo = two ? rest & (rest - 1) : rest;
+      pstage = !two ? next : next + 1 == NSTG ? 0 : next + 1;
+      issued += two ? 2 : 1;
+      want -= two ? 2 : 1;
     }
-    if (lane == __ffs(todo) - 1) {
-      mbar_arrive_expect_tx(&bar[pstage], REC);
-      bulk_load(ring + pstage * REC, src, REC, &bar[pstage], pol);
-    }
-    todo &= todo - 1;
-    pstage = pstage + 1 == NSTG ? 0 : pstage + 1;
-    ++issued;
   };
-  for (int i = 0; i < NSTG; ++i) issue();
+
+  bool primed = false;  // the ring's first fill goes out behind the first unit's q loads
 
   const float sl2 = P.a.scale * kLog2e;
   const float cap2 = P.a.mods.softcap * kLog2e, two_over = MOD ? 2.f / P.a.mods.softcap : 0.f;
@@ -445,6 +455,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
             }
           }
         }
+      if (!primed) {
+        primed = true;
+#pragma unroll 1
+        for (int i = 0; i < NSTG; ++i) issue(1);
+      }
       float top = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -517,36 +532,48 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
       // first record as keys that no row sees.
       int kb[TP];
       int n = 0;
+      if (!MOD && TP == 2) {  // live pages are the first ones
+        kb[0] = k * PAGE;
+        if (kb[0] > cc.hi_max) continue;
+        const bool two = k + 1 < cc.k1 && kb[0] + PAGE <= cc.hi_max;
+        kb[TP - 1] = two ? kb[0] + PAGE : 0x7fffff00;
+        n = two ? 2 : 1;
+      } else {
 #pragma unroll
-      for (int u = 0; u < TP; ++u) {
-        kb[u] = 0x7fffff00;
-        const int pg = cc.page(k + u);
-        if (k + u < cc.k1 && cc.live(pg)) {
-          if (TP == 2 && n == 0) kb[0] = pg * PAGE;
-          else kb[u] = pg * PAGE;
-          ++n;
+        for (int u = 0; u < TP; ++u) {
+          kb[u] = 0x7fffff00;
+          const int pg = cc.page(k + u);
+          if (k + u < cc.k1 && cc.live(pg)) {
+            if (TP == 2 && n == 0) kb[0] = pg * PAGE;
+            else kb[u] = pg * PAGE;
+            ++n;
+          }
         }
+        if (n == 0) continue;
       }
-      if (n == 0) continue;
+      const bool wrap = stage + 1 == NSTG;
+      const int st1 = wrap ? 0 : stage + 1;
+      const uint32_t ph1 = phase ^ (wrap ? 1u : 0u);
       uint32_t rec[TP];
-#pragma unroll
-      for (int u = 0; u < TP; ++u) {
-        rec[u] = u < n ? ring + stage * REC : rec[0];
-        if (u < n) {
-          if (!__all_sync(0xffffffffu, mbar_try_wait(&bar[stage], phase))) {
-            if (!dead && !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT)) dead = true;
-            dead = __any_sync(0xffffffffu, dead);
-          }
-          if (!dead) {
-            ++taken;
-            if (++stage == NSTG) {
-              stage = 0;
-              phase ^= 1u;
-            }
-          }
+      rec[0] = ring + stage * REC;
+      if (TP == 2) rec[TP - 1] = n == 2 ? ring + st1 * REC : rec[0];
+      bool here = mbar_try_wait(&bar[stage], phase);
+      if (TP == 2 && n == 2) here = here && mbar_try_wait(&bar[st1], ph1);
+      if (!__all_sync(0xffffffffu, here)) {
+        if (!dead) {
+          dead = !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT);
+          if (TP == 2 && n == 2 && !dead) dead = !mbar_wait_bounded(&bar[st1], ph1, WAIT_LIMIT);
         }
+        dead = __any_sync(0xffffffffu, dead);
       }
       if (dead) continue;
+      taken += n;
+      stage = st1;
+      phase = ph1;
+      if (TP == 2 && n == 2 && ++stage == NSTG) {
+        stage = 0;
+        phase ^= 1u;
+      }
 
       // ---------------------------------------------------------- S^T = K Q^T
       // At NT = 1 two accumulators halve the dependent chain.
@@ -759,7 +786,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
           }
         }
       __syncwarp();
-      for (int u = 0; u < n; ++u) issue();
+      issue(n);
     }
 
     // --------------------------------------------------- join the four warps' parts
@@ -842,7 +869,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
             T* dst = static_cast<T*>(P.a.out) +
                      (int64_t)map_row(P.a, g.q_start + div_g(P, rr)) * P.a.o_sr +
                      (int64_t)(cc.h * P.G + mod_g(P, rr)) * P.a.o_sh + col;
-            T e[4] = {from_f32<T>(a.x * inv), from_f32<T>(a.y * inv), from_f32<T>(a.z * inv),
+            alignas(16) T e[4] = {from_f32<T>(a.x * inv), from_f32<T>(a.y * inv), from_f32<T>(a.z * inv),
                       from_f32<T>(a.w * inv)};
             if (P.vec) {
               if constexpr (sizeof(T) == 2)
@@ -873,60 +900,81 @@ __global__ void __launch_bounds__(THREADS, Cfg<T, D, NT>::MINB)
   }
 }
 
-// Joins the partials of units that range borders cut (log-sum-exp identity), one
-// CTA per unit, in range order; zeros for rows of sequences without any visible page.
+// Joins the partials of units that range borders cut (log-sum-exp identity), one CTA per
+// unit, in range order; zeros for rows of sequences without any visible page.  Bound by
+// latency: a thread owns one float4 of a row and loads a batch of parts at once.
+constexpr int JOIN_THREADS = 256, JOIN_BATCH = 8;
+
 template <typename T, int D, int NT, bool MOD>
-__global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ Params P,
-                                                       int ranges) {
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Params P,
+                                                            int ranges) {
   constexpr int R = 8 * NT;
   grid_dependency_wait();
   const int s = blockIdx.y, u = blockIdx.x;
+  const uint32_t total = (uint32_t)__ldcg(P.prefix + P.a.num_seqs);
+  const uint32_t first = (uint32_t)__ldcg(P.prefix + s);
   const Geo g = seq_geo<MOD>(P, s, R, false);
-  const int rt = u / P.a.hkv, h = u % P.a.hkv;
+  const int rt = P.RT == 1 ? 0 : u / P.a.hkv, h = u - rt * P.a.hkv;
   if (rt >= g.nrt) return;
   int c0 = 0, c1 = 0;
-  Split S;
   if (g.n > 0) {
-    S = make_split((uint32_t)P.prefix[P.a.num_seqs], ranges, P.min_tiles);
-    const uint32_t start = (uint32_t)P.prefix[s] + (uint32_t)u * g.n;
+    const Split S = make_split(total, ranges, P.min_tiles);
+    const uint32_t start = first + (uint32_t)u * g.n;
     c0 = S.owner(start);
     c1 = S.owner(start + g.n - 1);
     if (c0 == c1) return;  // written whole
   }
-  for (int idx = threadIdx.x; idx < R * (D / 4); idx += THREADS) {
+  for (int idx = threadIdx.x; idx < R * (D / 4); idx += JOIN_THREADS) {
     const int row = idx / (D / 4), col = (idx % (D / 4)) * 4;
     const int rr = rt * R + row;
     if (rr >= g.q_len * P.G) break;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-    if (g.n > 0) {
-      auto slot = [&](int c) {
-        return P.part + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * P.part_floats;
-      };
-      float M = -INFINITY;
-#pragma unroll 8
-      for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(slot(c) + R * D + row));
-#pragma unroll 4
-      for (int c = c0; c <= c1; ++c) {
-        const float* sl = slot(c);
-        const float mc = __ldcg(sl + R * D + row), lc = __ldcg(sl + R * D + R + row);
-        const float4 b = __ldcg(reinterpret_cast<const float4*>(sl + row * D + col));
-        const float f = mc == -INFINITY ? 0.f : fast_exp2(mc - M);
-        L += mc == -INFINITY ? lc : lc * f;
-        a.x = fmaf(b.x, f, a.x);
-        a.y = fmaf(b.y, f, a.y);
-        a.z = fmaf(b.z, f, a.z);
-        a.w = fmaf(b.w, f, a.w);
+    float L = 0.f, M = -INFINITY;
+    for (int c = c0; g.n > 0 && c <= c1; c += JOIN_BATCH) {
+      float m[JOIN_BATCH], l[JOIN_BATCH];
+      float4 b[JOIN_BATCH];
+#pragma unroll
+      for (int i = 0; i < JOIN_BATCH; ++i) {
+        const int ci = min(c + i, c1);
+        const float* sl = P.part + ((int64_t)ci * 2 + (ci == c0 ? 1 : 0)) * P.part_floats;
+        m[i] = __ldcg(sl + R * D + row);
+        l[i] = __ldcg(sl + R * D + R + row);
+        b[i] = __ldcg(reinterpret_cast<const float4*>(sl + row * D + col));
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < JOIN_BATCH; ++i) top = fmaxf(top, m[i]);
+      const float f0 = M == -INFINITY ? 0.f : fast_exp2(M - top);
+      L *= f0;
+      a.x *= f0;
+      a.y *= f0;
+      a.z *= f0;
+      a.w *= f0;
+      M = top;
+#pragma unroll
+      for (int i = 0; i < JOIN_BATCH; ++i) {
+        if (c + i > c1) break;
+        const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - top);
+        L += m[i] == -INFINITY ? l[i] : l[i] * f;  // (a row of NaN scores has no maximum)
+        a.x = fmaf(b[i].x, f, a.x);
+        a.y = fmaf(b[i].y, f, a.y);
+        a.z = fmaf(b[i].z, f, a.z);
+        a.w = fmaf(b[i].w, f, a.w);
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     T* dst = static_cast<T*>(P.a.out) +
              (int64_t)map_row(P.a, g.q_start + div_g(P, rr)) * P.a.o_sr +
              (int64_t)(h * P.G + mod_g(P, rr)) * P.a.o_sh + col;
-    dst[0] = from_f32<T>(a.x * inv);
-    dst[1] = from_f32<T>(a.y * inv);
-    dst[2] = from_f32<T>(a.z * inv);
-    dst[3] = from_f32<T>(a.w * inv);
+    alignas(16) T e[4] = {from_f32<T>(a.x * inv), from_f32<T>(a.y * inv),
+                          from_f32<T>(a.z * inv), from_f32<T>(a.w * inv)};
+    if (P.vec) {
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(e);
+      else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[i] = e[i];
+    }
   }
 }
 
@@ -1146,6 +1194,7 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
         cudaError_t e = cudaLaunchKernelEx(&cfg, Kn::attn, P);
         if (e == cudaSuccess) {
           cfg.gridDim = dim3((unsigned)(pl.rt * P.a.hkv), (unsigned)P.a.num_seqs);
+          cfg.blockDim = dim3(q4a::JOIN_THREADS);
           cfg.dynamicSmemBytes = 0;
           e = cudaLaunchKernelEx(&cfg, Kn::join, P, pl.ranges);
         }
