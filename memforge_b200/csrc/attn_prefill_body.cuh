@@ -397,63 +397,67 @@ MF_DEVINL void q4_load(const Params& P, const int* prefix, const uint16_t* order
 }
 
 // The Q tile of one item, by the K warps (ts: thread of the 128; 16 lanes a row, 16 rows a
-// warp in two batches of 8): rows in fp16, times the power of two that brings a row's largest
-// element to [2^14, 2^15) (exact for bf16 and fp16 elements down to 2^-28 of it); its inverse
-// goes to the softmax.  Rows without a query are zeros.
-template <typename T>
-struct QTile {
-  static constexpr int U = BM / (2 * Q4_CW) / 2;
-  uint4 raw[U];
+// warp): rows in fp16, times the power of two that brings a row's largest element to
+// [2^14, 2^15) (exact for bf16 and fp16 elements down to 2^-28 of it); its inverse goes to the
+// softmax.  Rows without a query are zeros.  The rows are copied asynchronously to their places
+// in the tile and converted there by the threads that copied them, in rolled loops: code that
+// runs once an item comes from far in the instruction cache, so less of it is faster (unrolled
+// over registers this took 10 us an item).
+MF_DEVINL int q4_q_row(int it, int ts) { return (it * Q4_CW + (ts >> 5)) * 2 + ((ts & 31) >> 4); }
 
-  MF_DEVINL static int row(int b, int u, int ts) {
-    return ((b * U + u) * Q4_CW + (ts >> 5)) * 2 + ((ts & 31) >> 4);
-  }
-  MF_DEVINL void load(const Params& P, const Item& I, int b, int ts) {
-    const int rows = positions_per_tile(P.G) * P.G;
-    const uint32_t inv = 65536u / (uint32_t)P.G + 1u;  // r / G = r * inv >> 16 for r < 128
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = row(b, u, ts);
-      const int in = (int)((uint32_t)r * inv >> 16), pos = I.pos0 + in;
-      raw[u] = make_uint4(0, 0, 0, 0);
-      if (r < rows && pos < I.q_len) {
-        const T* p = static_cast<const T*>(P.a.q) +
-                     (int64_t)map_row(P.a, I.q_start + pos) * P.a.q_sr +
-                     (int64_t)(I.h * P.G + (r - in * P.G)) * P.a.q_sh + (ts & 15) * 8;
-        if (P.vec) {
-          raw[u] = __ldg(reinterpret_cast<const uint4*>(p));
-        } else {
-          const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
-          raw[u] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                              e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-        }
+template <typename T>
+MF_DEVINL void q4_stage_q(const Params& P, const Item& I, uint32_t tile, float* qs, int ts) {
+  const int c = ts & 15;
+  const int rows = positions_per_tile(P.G) * P.G;
+  const uint32_t inv = 65536u / (uint32_t)P.G + 1u;  // r / G = r * inv >> 16 for r < 128
+  const T* q = static_cast<const T*>(P.a.q) + c * 8;
+#pragma unroll 1
+  for (int it = 0; it < BM / (2 * Q4_CW); ++it) {
+    const int r = q4_q_row(it, ts);
+    const int in = (int)((uint32_t)r * inv >> 16), pos = I.pos0 + in;
+    const uint32_t dst = chunk_at(tile, r, c);
+    if (r < rows && pos < I.q_len) {
+      const T* p = q + (int64_t)map_row(P.a, I.q_start + pos) * P.a.q_sr +
+                   (int64_t)(I.h * P.G + (r - in * P.G)) * P.a.q_sh;
+      if (P.vec) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
+      } else {
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+        sts128(dst, e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+               e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
       }
+    } else {
+      sts128(dst, 0, 0, 0, 0);
     }
   }
-  MF_DEVINL void store(const Params& P, int b, uint32_t tile, float* qs, int ts) {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+  for (int it = 0; it < BM / (2 * Q4_CW); ++it) {
+    const int r = q4_q_row(it, ts);
+    const uint32_t dst = chunk_at(tile, r, c);
+    uint32_t raw[4];
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3])
+                 : "r"(dst)
+                 : "memory");
+    const T* t = reinterpret_cast<const T*>(raw);
+    float x[8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = row(b, u, ts);
-      const T* t = reinterpret_cast<const T*>(&raw[u]);
-      float x[8];
+    for (int e = 0; e < 8; ++e) x[e] = Elt<T>::to_f32(t[e]);
+    // (a NaN is passed over; with an infinity the row's output is NaN whatever the factor)
+    float top = fmaxf(fmax3f(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])),
+                      fmax3f(fabsf(x[3]), fabsf(x[4]), fmax3f(fabsf(x[5]), fabsf(x[6]), fabsf(x[7]))));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = Elt<T>::to_f32(t[e]);
-      // (a NaN is passed over; with an infinity the row's output is NaN whatever the factor)
-      float top = fmaxf(fmax3f(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])),
-                        fmax3f(fabsf(x[3]), fabsf(x[4]), fmax3f(fabsf(x[5]), fabsf(x[6]), fabsf(x[7]))));
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int ex = (int)(__float_as_uint(top) >> 23);
+    const float mul = __uint_as_float((uint32_t)min(max(268 - ex, 1), 240) << 23);
+    if (c == 0) qs[r] = 2.f * P.scale_log2 / mul;
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int ex = (int)(__float_as_uint(top) >> 23);
-      const float mul = __uint_as_float((uint32_t)min(max(268 - ex, 1), 240) << 23);
-      if ((ts & 15) == 0) qs[r] = 2.f * P.scale_log2 / mul;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= mul;
-      sts128(chunk_at(tile, r, ts & 15), Mma<__half>::pack(x[0], x[4]),
-             Mma<__half>::pack(x[1], x[5]), Mma<__half>::pack(x[2], x[6]),
-             Mma<__half>::pack(x[3], x[7]));
-    }
+    for (int e = 0; e < 8; ++e) x[e] *= mul;
+    sts128(dst, Mma<__half>::pack(x[0], x[4]), Mma<__half>::pack(x[1], x[5]),
+           Mma<__half>::pack(x[2], x[6]), Mma<__half>::pack(x[3], x[7]));
   }
-};
+}
 
 // K or V of every tile, by four warps; ts: thread of the 128, which take the pages of a tile
 // two at a time.  The K warps bring an item's Q first.  Codes become n * scale + base
@@ -573,19 +577,14 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
       if constexpr (!V) {
         if (j == 0) {
           // The item's Q, once the previous item's last S is done: after the first K tile, which
-          // only waited for a free stage, and with half the rows under way during the wait.
-          QTile<T> Q;
-          Q.load(P, I, 0, ts0);
+          // only waited for a free stage.
           const bool free = ic == 0 || mbar_wait_bounded(&bar[B_QEMPTY], (ic - 1) & 1, WAIT_LIMIT);
           if (!__all_sync(0xffffffffu, free && !*abort_flag)) {
             if (!free) set_err(P.a.err, MF_ERR_TIMEOUT);
             *abort_flag = 1;
             return;
           }
-          float* qrow = qs + (ic & 3) * BM;
-          Q.store(P, 0, base + OFF_Q, qrow, ts0);
-          Q.load(P, I, 1, ts0);
-          Q.store(P, 1, base + OFF_Q, qrow, ts0);
+          q4_stage_q<T>(P, I, base + OFF_Q, qs + (ic & 3) * BM, ts0);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar[B_QFULL]);

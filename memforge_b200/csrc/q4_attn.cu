@@ -984,8 +984,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
 
 namespace {
 
-// Rows per kv head up to which mma.sync keeps a run when the tcgen05 kernel could have it.
+// Which kernel takes a call's longest runs (the shortest, up to ROWS_CAP rows per kv head, stay
+// with mma.sync).  Per 128 keys, mma.sync spends about 10 ns of the whole GPU on a 16-row tile
+// of one head, and cuts long contexts over the SMs; the tcgen05 kernel 2.2 us of one SM on a
+// 128-row tile, whole contexts at a time, so ragged batches wait for their longest (half as
+// much again).  25 rows of 16 sequences, 8 heads: 64 us against 88.
 constexpr int ROWS_CAP = 32;
+bool chunks_win(int64_t rows, int64_t heads, int sms) {
+  const int64_t waves = (heads * ((rows + 127) / 128) + sms - 1) / std::max(sms, 1);
+  return rows > ROWS_CAP && heads * ((rows + 15) / 16) >= 340 * waves;
+}
 
 struct Plan {
   bool chunks, tiles;  // launch the tcgen05 kernel; launch the mma.sync kernel
@@ -995,13 +1003,10 @@ struct Plan {
   int part_floats;
 };
 
-// Row tiles: 8 rows while a run has no more (decode: most CTAs per SM), else 16 or
-// 32, which read the cache once for that many rows; at D = 256 and in fp32 the
-// accumulators and q of more rows would not fit the registers.
-int row_tile(int64_t rows, int d, bool f32) {
-  if (rows <= 8 || (f32 && d > 64)) return 1;
-  return rows <= 16 || d == 256 || f32 ? 2 : 4;
-}
+// Row tiles: 8 rows while a run has no more (decode), else 16.  A 32-row tile reads the
+// cache half as often but spills and leaves 8 warps on an SM: 25 rows at D = 128 took 71 us
+// with it and 64 us in two tiles of 16.  fp32's two-part q and P fit 16 rows at D = 64 only.
+int row_tile(int64_t rows, int d, bool f32) { return rows <= 8 || (f32 && d > 64) ? 1 : 2; }
 
 template <typename T_, int D_, int NT_, bool MOD_>
 struct Kern {
@@ -1019,9 +1024,7 @@ int with_tile(int d, int nt, F&& f) {
   if (d == 128 && nt == 1) return f(Kern<T, 128, 1, MOD>{});
   if (d == 256 && nt == 1) return f(Kern<T, 256, 1, MOD>{});
   if constexpr (!f32) {
-    if (d == 64 && nt == 4) return f(Kern<T, 64, 4, MOD>{});
     if (d == 128 && nt == 2) return f(Kern<T, 128, 2, MOD>{});
-    if (d == 128 && nt == 4) return f(Kern<T, 128, 4, MOD>{});
     if (d == 256 && nt == 2) return f(Kern<T, 256, 2, MOD>{});
   }
   return fail(MF_EUNSUPPORTED, "q4 attention: no kernel for this head_dim and dtype");
@@ -1104,7 +1107,7 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
 Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
   Plan pl{};
   int64_t rows = (int64_t)P.a.max_q_len * P.G;
-  pl.chunks = rows > ROWS_CAP && q4_prefill_serves(P.a, dt);
+  pl.chunks = chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
   pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
   if (!pl.tiles) return pl;
   if (pl.chunks) {
