@@ -9,6 +9,8 @@ these modules keep MemForge's operator API so they drop in for it:
 * ``varlen_attention``                 — ``paged_attention_varlen[_materialised]``
 * ``paged_decode``                     — ``paged_decode_attention`` (Triton signature)
 * ``paged_attention``                  — standalone ``PagedKVCache`` / ``PagedAttention``
+* ``scored_attention``                 — capped, biased, windowed and prefix attention
+* ``quant_cache``                      — the 4-bit KV cache: ``Q4KVPool`` and its operators
 * ``attention_backend``                — the transformers registry function
 * ``speculative``                      — verify over a side window + confirmed-prefix commit
 * ``kv_shard``                         — KV-head sharding across GPUs with an NCCL all-gather

@@ -21,6 +21,9 @@ How this one works:
 * A binding's kernel metadata (int32 tables, row offsets, key counts, row order)
   is built on its first use and uploaded once; every later layer of the same
   forward pass reuses the device copy.
+* Scores are modified as the model asks: ``softcap`` and ``sliding_window`` reach the kernel
+  (``scored_attention``).  Pools of 4-bit rows (``quant_cache.Q4KVPool``) serve bound calls
+  like any other pool.
 * ``graph_attention_context`` binds a batched decode step whose tables and
   lengths are device tensors (the graphed decoder captures it in a CUDA graph).
 * Outside any binding, the handed ``key``/``value`` are first written into a
@@ -135,7 +138,7 @@ class _VarlenBinding:
         if self._meta is None:
             plan, cu, kv, row_map, index = _varlen_plan(
                 len(self.seq_ids), self.block_tables, self.seq_ids, self.positions,
-                self.pool.block_size, num_heads, self.pool.key_pool.shape[3], device)
+                self.pool.block_size, num_heads, self.pool.spec.num_kv_heads, device)
             tables = _varlen_tables(plan, self.block_tables, index, device)
             self._meta = _DeviceRows(tables, cu, kv, row_map, plan.max_q_len, plan.total,
                                      q_per_seq=plan.uniform_q)
@@ -210,15 +213,26 @@ def any_binding_active() -> bool:
 
 # ------------------------------------------------------------ the function
 
-def _run(query_rows, out_rows, pool, layer_idx, meta: _DeviceRows, scale, causal=True):
+def _run(query_rows, out_rows, pool, layer_idx, meta: _DeviceRows, scale, mods):
     if meta.q_per_seq:
-        K.paged_attention(query_rows, out_rows, pool.key_pool[layer_idx],
-                          pool.value_pool[layer_idx], meta.tables, meta.kv,
-                          q_per_seq=meta.q_per_seq, scale=scale, causal=causal)
+        pool.attend(layer_idx, query_rows, out_rows, meta.tables, meta.kv,
+                    q_per_seq=meta.q_per_seq, scale=scale, **mods)
     else:
-        K.paged_attention(query_rows, out_rows, pool.key_pool[layer_idx],
-                          pool.value_pool[layer_idx], meta.tables, meta.kv, cu_seqlens_q=meta.cu,
-                          max_q_len=meta.max_q, scale=scale, causal=causal, row_map=meta.row_map)
+        pool.attend(layer_idx, query_rows, out_rows, meta.tables, meta.kv, cu_seqlens_q=meta.cu,
+                    max_q_len=meta.max_q, scale=scale, row_map=meta.row_map, **mods)
+
+
+def _score_mods(kwargs) -> dict:
+    """
+    The score modifiers a model hands its attention function: ``softcap`` (scores capped
+    by a tanh) and ``sliding_window`` (keys at most that many positions back).
+    """
+    mods = {}
+    if kwargs.get("softcap"):
+        mods["softcap"] = float(kwargs["softcap"])
+    if kwargs.get("sliding_window"):
+        mods["window"] = int(kwargs["sliding_window"])
+    return mods
 
 
 def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
@@ -228,7 +242,9 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
     """
     ``query`` ``(B, Hq, q_len, D)``; returns ``((B, q_len, Hq, D), None)``.
     Bound calls read K/V from the pool; unbound calls attend to ``key``/``value``.
+    ``softcap`` and ``sliding_window`` among the keywords are honoured.
     """
+    mods = _score_mods(kwargs)
     if dropout and getattr(module, "training", False):
         raise NotImplementedError("memforge_paged serves inference only (dropout > 0)")
     head_dim = query.shape[-1]
@@ -243,10 +259,8 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
         if q_len != 1:
             raise ValueError(f"a graphed decode step has one query row per sequence, got "
                              f"{q_len}")
-        pool = graph.pool
-        K.paged_attention(query[:, :, 0], out[:, 0], pool.key_pool[module.layer_idx],
-                          pool.value_pool[module.layer_idx], graph.tables, graph.ctx,
-                          q_per_seq=1, scale=scale, causal=True)
+        graph.pool.attend(module.layer_idx, query[:, :, 0], out[:, 0], graph.tables, graph.ctx,
+                          q_per_seq=1, scale=scale, causal=True, **mods)
         graph.used += 1
         return out, None
 
@@ -256,7 +270,8 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
             raise ValueError(f"varlen pass expected one packed row of {len(varlen.seq_ids)} "
                              f"tokens, got {tuple(query.shape)}")
         meta = varlen.rows(Hq, query.device)
-        _run(query[0].transpose(0, 1), out[0], varlen.pool, module.layer_idx, meta, scale)
+        _run(query[0].transpose(0, 1), out[0], varlen.pool, module.layer_idx, meta, scale,
+             mods)
         varlen.used += 1
         return out, None
 
@@ -265,14 +280,15 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
         if B != 1:
             raise ValueError(f"a paged cache binding is one sequence; got batch {B}")
         meta = binding.rows(q_len, query.device)
-        _run(query[0].transpose(0, 1), out[0], binding.pool, module.layer_idx, meta, scale)
+        _run(query[0].transpose(0, 1), out[0], binding.pool, module.layer_idx, meta, scale,
+             mods)
         binding.used += 1
         return out, None
 
-    return _unbound(module, query, key, value, attention_mask, scale, out), None
+    return _unbound(module, query, key, value, attention_mask, scale, out, mods), None
 
 
-def _unbound(module, query, key, value, attention_mask, scale, out):
+def _unbound(module, query, key, value, attention_mask, scale, out, mods):
     """Stage the handed K/V into a transient paged pool, then run the same kernel."""
     B, Hq, q_len, D = query.shape
     Hkv, kv_len = key.shape[1], key.shape[2]
@@ -291,7 +307,7 @@ def _unbound(module, query, key, value, attention_mask, scale, out):
     kv = torch.full((B,), kv_len, device=query.device, dtype=torch.int32)
     rows = query.transpose(1, 2).reshape(B * q_len, Hq, D)
     K.paged_attention(rows, out.view(B * q_len, Hq, D), pool_k, pool_v, tables, kv,
-                      q_per_seq=q_len, scale=scale, causal=causal)
+                      q_per_seq=q_len, scale=scale, causal=causal, **mods)
     return out
 
 

@@ -29,7 +29,6 @@ from typing import Dict, Optional, Sequence
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
-from . import _kernels as K
 from . import attention_backend as AB
 
 
@@ -48,8 +47,7 @@ class _GraphLayer(CacheLayerMixin):
         o, l = self.owner, self.layer_idx
         b = o._b
         # (B, H, 1, D) -> (B, H, D) rows at each row's slot, this layer's pool
-        K.reshape_and_cache(key_states[:, :, 0], value_states[:, :, 0], o.pool.key_pool[l],
-                            o.pool.value_pool[l], o._slots[:b])
+        o.pool.write_rows(l, key_states[:, :, 0], value_states[:, :, 0], o._slots[:b])
         return key_states, value_states
 
     def get_seq_length(self) -> int:
@@ -78,7 +76,7 @@ class GraphedPagedDecoder:
         if not AB.register():
             raise RuntimeError("graphed paged decode needs the transformers attention registry")
         self.model, self.pool = model, pool
-        self.device = torch.device(pool.key_pool.device)
+        self.device = torch.device(pool.device)
         if self.device.type != "cuda":
             raise ValueError("graphed paged decode needs a CUDA device")
         self.bs = pool.block_size

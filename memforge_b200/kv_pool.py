@@ -14,6 +14,7 @@ from typing import List, Tuple
 
 import torch
 
+from . import _kernels as K
 from . import paged_gather
 
 
@@ -112,6 +113,22 @@ class PagedKVPool:
         """``kv_pool.py:181-192``: one scatter kernel for K and V."""
         paged_gather.scatter_kv(self.key_pool, self.value_pool, layer_idx, flat_index, keys,
                                 values, self.block_size)
+
+    @property
+    def device(self) -> torch.device:
+        return self.key_pool.device
+
+    def write_rows(self, layer_idx: int, keys: torch.Tensor, values: torch.Tensor,
+                   slots: torch.Tensor) -> None:
+        """Scatter ``(T, H, D)`` rows at ``slots`` (device tensor; graph safe)."""
+        K.reshape_and_cache(keys, values, self.key_pool[layer_idx], self.value_pool[layer_idx],
+                            slots)
+
+    def attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor,
+               block_tables: torch.Tensor, kv_lens: torch.Tensor, **how) -> torch.Tensor:
+        """``_kernels.paged_attention`` of ``(rows, Hq, D)`` queries over one layer."""
+        return K.paged_attention(q, out, self.key_pool[layer_idx], self.value_pool[layer_idx],
+                                 block_tables, kv_lens, **how)
 
     def zero_(self) -> None:
         self.key_pool.zero_()

@@ -271,7 +271,7 @@ class VarlenPackedCache(Cache):
         tables a slot named by two sequences is rejected too.
         """
         bs = self.pool.block_size
-        device = self.pool.key_pool.device
+        device = self.pool.device
         sizes = [int(t.numel()) if hasattr(t, "numel") else len(t) for t in self.block_tables]
         offs = [0]
         for n in sizes:

@@ -95,6 +95,8 @@ class Q4KVPool(PagedKVPool):
     def __init__(self, spec: ModelKVSpec, num_blocks: int, block_size: int = BLOCK_SIZE):
         if block_size != BLOCK_SIZE:
             raise ValueError(f"the 4-bit cache has blocks of {BLOCK_SIZE} tokens, got {block_size}")
+        if spec.dtype not in K.DTYPES:
+            raise TypeError(f"unsupported dtype {spec.dtype}; expected float32, float16 or bfloat16")
         self.spec = spec
         self.num_blocks = num_blocks
         self.block_size = block_size
@@ -135,6 +137,10 @@ class Q4KVPool(PagedKVPool):
                block_tables: torch.Tensor, kv_lens: torch.Tensor, **how) -> torch.Tensor:
         return K.q4_paged_attention(q, out, self.pool, block_tables, kv_lens, layer=layer_idx,
                                     **how)
+
+    def copy_blocks(self, pairs: torch.Tensor) -> None:
+        """Copy block src -> dst in every layer; ``pairs`` int32 ``[n, 2]`` on the device."""
+        K.copy_blocks(self.pool, self.pool, pairs)   # K and V share a record
 
     def zero_(self) -> None:
         self.pool.zero_()

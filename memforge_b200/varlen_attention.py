@@ -87,27 +87,25 @@ def _tables(plan: VarlenPlan, block_tables, index, device) -> torch.Tensor:
     return torch.from_numpy(plan.host_tables(block_tables)).to(device)
 
 
-def _run(query, key_layer, value_layer, block_tables, seq_ids, positions, scale, block_size):
-    K.require_cuda("paged_attention_varlen", query, key_layer, value_layer)
+def _run(query, attend, num_kv_heads, pool_block, block_tables, seq_ids, positions, scale,
+         block_size):
     if query.shape[0] != 1:
         raise ValueError(f"expected a packed batch of 1, got {tuple(query.shape)}")
     plan, cu, kv, row_map, index = _plan(query.shape[2], block_tables, seq_ids, positions,
-                                         block_size, query.shape[1], key_layer.shape[2],
+                                         block_size, query.shape[1], num_kv_heads,
                                          query.device)
-    if key_layer.shape[1] != block_size:
-        raise ValueError(f"pool block size {key_layer.shape[1]} does not match {block_size}")
+    if pool_block != block_size:
+        raise ValueError(f"pool block size {pool_block} does not match {block_size}")
     head_dim = query.shape[3]
     scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
     tables = _tables(plan, block_tables, index, query.device)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if plan.uniform_q:
-        K.paged_attention(query[0].transpose(0, 1), out[0].transpose(0, 1), key_layer,
-                          value_layer, tables, kv, q_per_seq=plan.uniform_q, scale=scale,
-                          causal=True)
+        attend(query[0].transpose(0, 1), out[0].transpose(0, 1), tables, kv,
+               q_per_seq=plan.uniform_q, scale=scale, causal=True)
     else:
-        K.paged_attention(query[0].transpose(0, 1), out[0].transpose(0, 1), key_layer,
-                          value_layer, tables, kv, cu_seqlens_q=cu, max_q_len=plan.max_q_len,
-                          scale=scale, causal=True, row_map=row_map)
+        attend(query[0].transpose(0, 1), out[0].transpose(0, 1), tables, kv, cu_seqlens_q=cu,
+               max_q_len=plan.max_q_len, scale=scale, causal=True, row_map=row_map)
     return out
 
 
@@ -121,7 +119,13 @@ def paged_attention_varlen(query: torch.Tensor, key_pool: torch.Tensor, value_po
     of ``block_tables[seq_ids[r]]``.  ``query`` is ``(1, H, T, D)``; the result
     has the same shape and dtype.
     """
-    return _run(query, key_pool[layer_idx], value_pool[layer_idx], block_tables, seq_ids,
+    key_layer, value_layer = key_pool[layer_idx], value_pool[layer_idx]
+    K.require_cuda("paged_attention_varlen", query, key_layer, value_layer)
+
+    def attend(q, out, tables, kv, **how):
+        K.paged_attention(q, out, key_layer, value_layer, tables, kv, **how)
+
+    return _run(query, attend, key_layer.shape[2], key_layer.shape[1], block_tables, seq_ids,
                 positions, scale, block_size)
 
 
@@ -130,8 +134,17 @@ def paged_attention_varlen_materialised(query: torch.Tensor, pool, layer_idx: in
                                         seq_ids: Sequence[int], positions: Sequence[int],
                                         scale: Optional[float] = None) -> torch.Tensor:
     """
-    Same function as ``paged_attention_varlen`` (``varlen_attention.py:291-395``).
+    Same function as ``paged_attention_varlen`` (``varlen_attention.py:291-395``), over a
+    ``PagedKVPool`` or a 4-bit ``Q4KVPool``.
     On B200 nothing is materialised: both names run the same kernel.
     """
-    return _run(query, pool.key_pool[layer_idx], pool.value_pool[layer_idx], block_tables,
-                seq_ids, positions, scale, pool.block_size)
+    if not hasattr(pool, "attend"):
+        return paged_attention_varlen(query, pool.key_pool, pool.value_pool, layer_idx,
+                                      block_tables, seq_ids, positions, pool.block_size, scale)
+    K.require_cuda("paged_attention_varlen", query)
+
+    def attend(q, out, tables, kv, **how):
+        pool.attend(layer_idx, q, out, tables, kv, **how)
+
+    return _run(query, attend, pool.spec.num_kv_heads, pool.block_size, block_tables, seq_ids,
+                positions, scale, pool.block_size)
