@@ -677,7 +677,7 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
     ws, nbytes = workspace_tensor, 0
     if ws is None:
         key = (dev.index, code, D, hq, hkv, num_seqs, most, width, cu_seqlens_q is None,
-               mods is None, rows == 0)
+               mods is None, rows, (a.q | a.out | 2 * (qs[0] | qs[1] | os_[0] | os_[1])) & 15)
         nbytes = _q4_need.get(key)
         if nbytes is None:
             nbytes = lib.mf_q4_paged_attention_workspace_size(a, dev.index)

@@ -186,8 +186,9 @@ struct Params {
   float scale_log2;
   uint32_t in_fmt;   // 0 = f16, 1 = bf16
   int window;        // 1: the last q_len keys of each sequence come from the window buffers
-  int width;         // Q4: entries of a block table's row
+  int width;         // Q4, EXP: entries of a block table's row
   int vec;           // Q4: q and out rows allow 16-byte accesses
+  const float* qs;   // EXP: per (row, query head), what scales S to log2 units
 };
 
 // Geometry of one work item (identical in every role).
@@ -220,7 +221,7 @@ MF_DEVINL int find_tile_seq(const int* prefix, int B, int t) {
 
 // Items run longest first: sequences by decreasing kv_len, and within a
 // sequence the last query tiles (which see the most keys) first.
-template <bool MOD, bool Q4>
+template <bool MOD, bool Q4>  // Q4: of a 4-bit cache (in either form)
 MF_DEVINL Item item_at(const Params& P, const int* prefix, const uint16_t* order, int B,
                        int it) {
   Item I;
@@ -594,12 +595,15 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
   }
 }
 
-// The kernel: Q, K and V tiles by TMA from a 16-bit pool (the five tensor maps), or with
-// Q4 converted by warps from a 4-bit pool (no maps; products and P in fp16).
-template <typename T, bool MOD, bool Q4>
+// The kernel: Q, K and V tiles by TMA from a 16-bit pool (the five tensor maps); with Q4
+// converted by warps from a 4-bit pool (no maps); with EXP by TMA from a 4-bit pool that was
+// expanded to fp16 beforehand (sequence s's page L at s * width + L, and q with it).  In the
+// latter two products and P are fp16, keys and values halved.
+template <typename T, bool MOD, bool Q4, bool EXP = false>
 MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv,
                             const CUtensorMap* tmwk, const CUtensorMap* tmwv, const Params& P) {
-  using PT = typename std::conditional<Q4, __half, T>::type;  // type of P
+  constexpr bool FOUR = Q4 || EXP;                              // of a 4-bit cache
+  using PT = typename std::conditional<FOUR, __half, T>::type;  // type of P
   constexpr int NTHR = Q4 ? Q4_THREADS : THREADS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
@@ -662,7 +666,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
     int tiles = 0;
     const int kvl = P.a.kv_lens[i];
     const bool mine = ql > 0 && (int64_t)ql * G > P.rows_cap;
-    if (Q4 && mine) {
+    if (FOUR && mine) {
       if (ql > P.a.max_q_len || kvl < 0) set_err(P.a.err, MF_ERR_LENGTH);
       if ((kvl + (int64_t)PAGE - 1) / PAGE > P.width) set_err(P.a.err, MF_ERR_TABLE);
       ql = min(ql, P.a.max_q_len);
@@ -763,7 +767,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
       uint32_t g = 0;
       int ic = 0;
       for (int k = 0; ok && snake_item(k) < items; ++k, ++ic) {
-        const Item I = item_at<MOD, Q4>(P, prefix, order, B, snake_item(k));
+        const Item I = item_at<MOD, FOUR>(P, prefix, order, B, snake_item(k));
         constexpr int NQ = q_buffers(Q4);
         const int qb = ic % NQ;
         if (!is_pv) ok = mbar_wait_bounded(&bar[B_QFULL + qb], (ic / NQ) & 1, WAIT_LIMIT);
@@ -875,8 +879,8 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[B_OFREE]);  // O may be overwritten
       if (pend_valid) {
-        const float inv = Q4 ? (l_tot == 0.f ? 0.f : 2.f / l_tot) : l_tot > 0.f ? 1.f / l_tot : 0.f;
-        if (Q4 && !P.vec) {
+        const float inv = FOUR ? (l_tot == 0.f ? 0.f : 2.f / l_tot) : l_tot > 0.f ? 1.f / l_tot : 0.f;
+        if (Q4 && !P.vec) {  // (EXP takes calls with 16-byte rows only)
 #pragma unroll
           for (int e = 0; e < 64; ++e) pend_row[e] = from_f32<T>(__uint_as_float(o[e]) * inv);
         } else
@@ -896,18 +900,20 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
     uint32_t g = 0;
     int ic = 0;
     for (int k = 0; ok && snake_item(k) < items; ++k, ++ic) {
-      const Item I = item_at<MOD, Q4>(P, prefix, order, B, snake_item(k));
+      const Item I = item_at<MOD, FOUR>(P, prefix, order, B, snake_item(k));
       const int pos = I.pos0 + row / G;  // query position of this row within the sequence
       const int gg = row % G;
       const bool row_valid = row < positions_per_tile(G) * G && pos < I.q_len;
       // Last visible key: causal over the context; with a window, every pool key
       // and, in the window tile, window keys 0..pos.
       const int limit = P.window ? I.pool_len - 1
-                        : Q4     ? min(P.a.causal ? I.win_start + pos : I.kv_len - 1, I.pool_len - 1)
+                        : FOUR   ? min(P.a.causal ? I.win_start + pos : I.kv_len - 1, I.pool_len - 1)
                                  : min(I.win_start + pos, I.kv_len - 1);
       const int row_lo =
           MOD && P.a.mods.window > 0 ? I.win_start + pos - P.a.mods.window + 1 : 0;
       const float slope = MOD && P.a.mods.slopes ? P.a.mods.slopes[I.h * G + gg] * kLog2e : 0.f;
+      const float item_sl2 =
+          EXP && row_valid ? __ldg(P.qs + (int64_t)(I.q_start + pos) * P.a.hq + I.h * G + gg) : 0.f;
       float m_seen = -INFINITY;  // reference max l_own is scaled to
       float l_own = 0.f;
       for (int j = 0; j < I.nt; ++j, ++g) {
@@ -924,7 +930,10 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
         for (int c = 0; c < CW / 32; ++c)
           tmem_ld32(tmem + COL_S + par * 128 + lane_off + c * 32,
                     reinterpret_cast<uint32_t*>(sv + c * 32));
-        if constexpr (Q4) {
+        if constexpr (EXP) {
+          raw_sl2 = item_sl2;
+          if (!transformed) sl2 = raw_sl2;
+        } else if constexpr (Q4) {
           raw_sl2 = reinterpret_cast<const float*>(gbase + off_qs())[(ic & 3) * BM + row];
           if (!transformed) sl2 = raw_sl2;
         }
@@ -1060,7 +1069,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
         // MOD: keys [dead0, dead1) lie behind every row's window.
         const int dead0 = MOD ? max(I.pfx - kbase, 0) : 0;
         const int dead1 = MOD ? min(I.lo - kbase, BN) : 0;
-        if (!Q4 && quarter == 0 && (loaded < BN || dead0 < dead1)) {
+        if (!Q4 && quarter == 0 && ((!EXP && loaded < BN) || dead0 < dead1)) {
           // Zero the V rows of those keys (whole 128-byte rows of both halves)
           // so p = 0 adds nothing even where a slot holds NaN.  This warp's
           // P-full arrival orders it before P V.
@@ -1102,7 +1111,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
       pend_valid = row_valid;
       const int out_row = I.q_start + (row_valid ? pos : 0);
       pend_row = static_cast<T*>(P.a.out) +
-                 (int64_t)(Q4 && row_valid ? map_row(P.a, out_row) : out_row) * P.a.o_sr +
+                 (int64_t)(FOUR && row_valid ? map_row(P.a, out_row) : out_row) * P.a.o_sr +
                  (int64_t)(I.h * G + gg) * P.a.o_sh + par * 64;
       pend_l = l_own;
       pend_m = m_seen;
@@ -1157,7 +1166,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
     const uint32_t ring = is_v ? off_v(Q4) : off_k(Q4);
     uint64_t* fullb = &bar[is_v ? B_VFULL : B_KFULL];
     uint64_t* emptyb = &bar[is_v ? B_PVDONE : B_SDONE];  // ring stage g % KS frees
-    const int nb = P.a.num_blocks;
+    const int nb = EXP ? P.a.num_seqs * P.width : P.a.num_blocks;
     const bool boxer = lane < 2 * (BN / PAGE);
     const int my_pg = lane >> 1, my_half = lane & 1;
     uint32_t g = 0;      // tiles started (all items)
@@ -1167,7 +1176,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
     for (int k = 0; run && snake_item(k) < items; ++k) {
       run = __shfl_sync(0xffffffffu, *abort_flag == 0, 0);
       if (!run) break;
-      const Item I = item_at<MOD, Q4>(P, prefix, order, B, snake_item(k));
+      const Item I = item_at<MOD, FOUR>(P, prefix, order, B, snake_item(k));
       if (!is_v) {
         const int qb = ic & 1;
         bool fine = true;
@@ -1193,8 +1202,8 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
       // Block id of this lane's page, loaded one tile ahead.  Out-of-table
       // pages use an out-of-range coordinate: TMA fills zeros.
       auto block_of = [&](int page) {
-        return boxer && page < pool_pages && I.template page_live<MOD>(page) ? __ldg(table + page)
-                                                                             : -1;
+        if (!boxer || page >= pool_pages || !I.template page_live<MOD>(page)) return -1;
+        return EXP ? I.s * P.width + page : __ldg(table + page);
       };
       int nxt = block_of(I.template tile<MOD>(0) * (BN / PAGE) + my_pg);
       for (int j = 0; j < I.nt; ++j, ++g) {

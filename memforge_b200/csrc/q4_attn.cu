@@ -997,6 +997,9 @@ bool chunks_win(int64_t rows, int64_t heads, int sms) {
 
 struct Plan {
   bool chunks, tiles;  // launch the tcgen05 kernel; launch the mma.sync kernel
+  bool expand;         // the tcgen05 kernel reads an expanded copy (at ws + expand_at)
+  size_t expand_at;
+  Q4Scratch scratch;
   int nt, ranges;
   int64_t rt;
   size_t prefix_bytes, ws_bytes;
@@ -1109,7 +1112,11 @@ Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
   int64_t rows = (int64_t)P.a.max_q_len * P.G;
   pl.chunks = chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
   pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
-  if (!pl.tiles) return pl;
+  pl.expand = pl.chunks && q4_expand_plan(P.a, P.width, P.vec, dt, pl.scratch);
+  if (!pl.tiles) {
+    if (pl.expand) pl.ws_bytes = pl.scratch.bytes;
+    return pl;
+  }
   if (pl.chunks) {
     P.rows_cap = ROWS_CAP;
     rows = std::min<int64_t>(rows, ROWS_CAP);
@@ -1130,6 +1137,10 @@ Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
   pl.part_floats = 8 * pl.nt * (P.a.d + 2);
   pl.prefix_bytes = ((size_t)(P.a.num_seqs + 1) * 4 + 255) & ~(size_t)255;
   pl.ws_bytes = pl.prefix_bytes + (size_t)pl.ranges * 2 * pl.part_floats * sizeof(float);
+  if (pl.expand) {
+    pl.expand_at = (pl.ws_bytes + 255) & ~(size_t)255;
+    pl.ws_bytes = pl.expand_at + pl.scratch.bytes;
+  }
   return pl;
 }
 
@@ -1160,15 +1171,18 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
   if (pl.tiles && (double)pl.rt * P.a.hkv * P.a.num_seqs * P.width >= 2147483648.0)
     return fail(MF_EUNSUPPORTED, "q4 attention: the tables could hold 2^31 or more (row tile, "
                                  "page) pairs");
-  if (pl.tiles && (!workspace || workspace_bytes < pl.ws_bytes ||
-                   (reinterpret_cast<uintptr_t>(workspace) & 15)))
+  if (pl.ws_bytes > 0 && (!workspace || workspace_bytes < pl.ws_bytes ||
+                          (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail(MF_EWORKSPACE, "q4 attention: workspace missing, misaligned or smaller than "
                                "mf_q4_paged_attention_workspace_size()");
   P.prefix = static_cast<int32_t*>(workspace);
   if (pl.tiles) P.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.prefix_bytes);
   P.part_floats = pl.part_floats;
   if (pl.chunks) {
-    const int rc2 = launch_q4_prefill(P.a, P.width, P.vec, P.rows_cap, args->dtype, s);
+    const int rc2 =
+        pl.expand ? launch_q4_expanded(P.a, P.width, P.rows_cap, args->dtype,
+                                       pl.scratch, static_cast<uint8_t*>(workspace) + pl.expand_at, s)
+                  : launch_q4_prefill(P.a, P.width, P.vec, P.rows_cap, args->dtype, s);
     if (rc2 != MF_OK || !pl.tiles) return rc2;
   }
   return with_kernel(

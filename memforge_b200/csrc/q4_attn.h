@@ -14,4 +14,15 @@ bool q4_prefill_serves(const AttnParams& a, mf_dtype dtype);
 int launch_q4_prefill(const AttnParams& a, int width, int vec, int rows_cap, mf_dtype dtype,
                       cudaStream_t stream);
 
+// The same over a copy of the cache that the call expands to fp16 in the workspace first:
+// faster where many row tiles read a key, at 512 bytes per token and kv head.
+struct Q4Scratch {
+  size_t q, scale, k, v, bytes;  // offsets, and their total
+};
+// The expanded form's workspace, or false where it does not serve (rows that are not 16-byte
+// aligned) or would exceed its limit.
+bool q4_expand_plan(const AttnParams& a, int width, int vec, mf_dtype dtype, Q4Scratch& sc);
+int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, mf_dtype dtype,
+                       const Q4Scratch& sc, uint8_t* ws, cudaStream_t stream);
+
 }  // namespace mf

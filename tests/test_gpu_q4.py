@@ -291,6 +291,37 @@ def test_long_runs(dtype, hq, hkv, ql):
     Case(50 + ql, dtype, hq, hkv, 128, [ql, ql + 127, ql + 128, 700], [ql] * 4).check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("mods", [dict(), dict(softcap=4.0), dict(window=130, prefix=[20, 300, 0]),
+                                  dict(slopes=True)])
+def test_runs_of_many_row_tiles(dtype, wide, mods):
+    """Runs of four row tiles and more read an expanded copy of the cache, unless the tables'
+    width would let it grow past its limit (then they convert as they go): both agree with the
+    definition, beside a short run and one without rows."""
+    c = Case(60, dtype, 8, 2, 128, [420, 300, 700], [200, 131, 512], **mods)
+    if wide:
+        t = np.full((3, 30000), -1, np.int32)
+        t[:, :c.tables.shape[1]] = c.tables
+        c.tables = t
+    c.check()
+    c = Case(61, dtype, 8, 2, 128, [420, 33, 50, 700], [300, 3, 0, 129])
+    c.check()
+
+
+def test_many_row_tiles_row_map_and_strides():
+    c = Case(62, "bf16", 8, 1, 128, [190, 220], [140, 133])
+    rows = 273
+    wide_q = torch.zeros((rows, 8, 131), dtype=torch.bfloat16, device="cuda")
+    perm = torch.from_numpy(rng(62).permutation(rows).astype(np.int32)).cuda()
+    wide_q[perm.long(), :, 1:129] = c.q_dev
+    wide_o = torch.full((rows, 8, 133), 5.0, dtype=torch.bfloat16, device="cuda")
+    c.run(q=wide_q[:, :, 1:129], out=wide_o[:, :, 2:130], row_map=perm)
+    want, tol = c.want()
+    got = wide_o[perm.long(), :, 2:130].double().cpu().numpy()
+    assert (np.abs(got - want) <= tol).all() and (wide_o[:, :, :2] == 5.0).all()
+
+
 def test_long_runs_non_causal_and_without_keys():
     Case(51, "bf16", 4, 2, 128, [150, 9], [70] * 2, causal=False).check()
     got = Case(52, "bf16", 4, 1, 128, [0, 20, 300], [60] * 3).check()
@@ -509,3 +540,40 @@ def test_write_then_attend_on_another_stream():
     o, _ = R.attention(c.q, rows, rows, c.scale, np.ones((1, 64), bool))
     tol = R.q4_tolerance("bf16", o, c.q, 15.0, 15.0, c.scale)
     assert (np.abs(out.double().cpu().numpy() - o) <= tol).all()
+
+
+@pytest.mark.parametrize("window", [1, 16, 127, 128, 129, 300])
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_row_tiles_windows_around_tiles(window, wide):
+    """Enough heads that the tensor-core kernels take the runs, expanded and converting."""
+    for mods in (dict(), dict(prefix=[130, 1, 600])):
+        c = Case(63, "bf16", 16, 4, 128, [500, 217, 640], [200] * 3, window=window, **mods)
+        if wide:
+            t = np.full((3, 15000), -1, np.int32)
+            t[:, :c.tables.shape[1]] = c.tables
+            c.tables = t
+        c.check()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_row_tiles_non_causal_without_keys_and_extremes(wide):
+    def run(c):
+        if wide:
+            t = np.full((len(c.kv_lens), 15000), -1, np.int32)
+            t[:, :c.tables.shape[1]] = c.tables
+            c.tables = t
+        return c.check()
+    run(Case(64, "bf16", 16, 4, 128, [150, 9, 400], [130] * 3, causal=False))
+    got = run(Case(65, "bf16", 16, 4, 128, [0, 20, 300], [160] * 3))
+    assert not got[:160].any() and not got[160:300].any() and got[300:320].any()
+    c = Case(66, "bf16", 16, 4, 128, [200, 200, 200], [140] * 3, q_scale=1e-6)
+    par = c.pool[:, :, 16 * 128:].view(np.float16).reshape(-1, 4, 2, 16, 2)
+    par[:, :, :, 0::3] = (8728.0, -65504.0)   # codes reach 65416
+    par[:, :, :, 1::3] = (0.5, 60000.0)
+    par[:, :, :, 2::3] = (2.0 ** -24, -2.0 ** -20)
+    run(c)
+
+
+def test_many_row_tiles_of_every_group_size():
+    for hq, hkv, ql in ((4, 4, 700), (28, 4, 100), (8, 4, 300), (80, 5, 40), (96, 2, 60)):
+        Case(67 + hq, "bf16", hq, hkv, 128, [ql + 5, ql + 300, ql], [ql] * 3).check()
