@@ -1180,9 +1180,9 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
   P.part_floats = pl.part_floats;
   if (pl.chunks) {
     const int rc2 =
-        pl.expand ? launch_q4_expanded(P.a, P.width, P.rows_cap, args->dtype,
-                                       pl.scratch, static_cast<uint8_t*>(workspace) + pl.expand_at, s)
-                  : launch_q4_prefill(P.a, P.width, P.vec, P.rows_cap, args->dtype, s);
+        pl.expand ? launch_q4_expanded(P.a, P.width, P.rows_cap, pl.scratch,
+                                       static_cast<uint8_t*>(workspace) + pl.expand_at, s)
+                  : launch_q4_prefill(P.a, P.width, P.vec, P.rows_cap, s);
     if (rc2 != MF_OK || !pl.tiles) return rc2;
   }
   return with_kernel(

@@ -11,7 +11,7 @@ bool q4_prefill_serves(const AttnParams& a, mf_dtype dtype);
 // Serves every sequence with more than rows_cap rows per kv head.  a.kp: the pool, a.sb /
 // a.sh its strides in bytes; width: entries of a block table's row; vec: q and out rows
 // allow 16-byte accesses.
-int launch_q4_prefill(const AttnParams& a, int width, int vec, int rows_cap, mf_dtype dtype,
+int launch_q4_prefill(const AttnParams& a, int width, int vec, int rows_cap,
                       cudaStream_t stream);
 
 // The same over a copy of the cache that the call expands to fp16 in the workspace first:
@@ -22,7 +22,7 @@ struct Q4Scratch {
 // The expanded form's workspace, or false where it does not serve (rows that are not 16-byte
 // aligned) or would exceed its limit.
 bool q4_expand_plan(const AttnParams& a, int width, int vec, mf_dtype dtype, Q4Scratch& sc);
-int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, mf_dtype dtype,
-                       const Q4Scratch& sc, uint8_t* ws, cudaStream_t stream);
+int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, const Q4Scratch& sc,
+                       uint8_t* ws, cudaStream_t stream);
 
 }  // namespace mf

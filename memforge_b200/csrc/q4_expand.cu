@@ -4,7 +4,7 @@
 //
 // The converting form of that kernel redoes the conversion for every 128-row tile, and its
 // converters' 3000 instructions a key tile share the SM with the softmax (913 us for four
-// ragged chunks of 300..2048 rows, 32/8 heads, where a 16-bit pool takes 564 us).  Expanding costs
+// ragged chunks of 300..2048 rows, 32/8 heads; 805 us in this form, 649 us from a 16-bit pool).  Expanding costs
 // 512 bytes of writes per token and kv head, once.  It is used from four row tiles on, while
 // the expanded copy (bounded by the tables' width) stays below SCRATCH_MAX.
 
@@ -195,8 +195,8 @@ bool q4_expand_plan(const AttnParams& a, int width, int vec, mf_dtype dtype, Q4S
   return true;
 }
 
-int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, mf_dtype dtype,
-                       const Q4Scratch& sc, uint8_t* ws, cudaStream_t stream) {
+int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, const Q4Scratch& sc,
+                       uint8_t* ws, cudaStream_t stream) {
   pf::Params P{};
   P.a = a;
   P.G = a.hq / a.hkv;
@@ -223,11 +223,8 @@ int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, mf_dtype dt
   const int64_t items = (int64_t)a.num_seqs * ((a.max_q_len + ppt - 1) / ppt) * a.hkv;
   const int64_t grid = std::min<int64_t>(items, current_sm_count());
   const bool mod = a.mods.any();
-  if (dtype == MF_BF16)
-    return mod ? pf::launch_expanded<__nv_bfloat16, true>(P, mq, mk, mv, q, scale, k, v, grid, stream)
-               : pf::launch_expanded<__nv_bfloat16, false>(P, mq, mk, mv, q, scale, k, v, grid, stream);
-  return mod ? pf::launch_expanded<__half, true>(P, mq, mk, mv, q, scale, k, v, grid, stream)
-             : pf::launch_expanded<__half, false>(P, mq, mk, mv, q, scale, k, v, grid, stream);
+  return mod ? pf::launch_expanded<__nv_bfloat16, true>(P, mq, mk, mv, q, scale, k, v, grid, stream)
+             : pf::launch_expanded<__nv_bfloat16, false>(P, mq, mk, mv, q, scale, k, v, grid, stream);
 }
 
 }  // namespace mf
