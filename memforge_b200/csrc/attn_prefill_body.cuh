@@ -461,12 +461,12 @@ MF_DEVINL void q4_stage_q(const Params& P, const Item& I, uint32_t tile, float* 
 }
 
 // K or V of every tile, by four warps; ts: thread of the 128, which take the pages of a tile
-// two at a time.  The K warps bring an item's Q first.  Codes become n * scale + base
-// halved, in fp16 (one rounding; halved so that no code of a row passes fp16's range; the
-// scores and the output take the factor back), stored as the swizzled tile the MMA reads. Keys without a token
-// (or behind every row's window) become zeros, whatever their slots hold.  K's dims stay in
-// the order the masks give inside each group of eight (0 4 1 5 2 6 3 7); the Q warps store
-// q in the same order.
+// two at a time.  The K warps bring an item's Q after its first K tile.  Codes become
+// n * scale + base halved, in fp16 (one rounding; halved so that no code of a row passes fp16's
+// range; the scores and the output take the factor back), stored as the swizzled tile the MMA
+// reads.  Keys without a token (or behind every row's window) become zeros, whatever their
+// slots hold.  K's dims stay in the order the masks give inside each group of eight
+// (0 4 1 5 2 6 3 7); q is stored in the same order.
 template <typename T, bool MOD, bool V>
 MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* order, int items,
                         uint32_t base, float* qs, uint64_t* bar, volatile int* abort_flag,

@@ -3,9 +3,9 @@
 // them by TMA (attn_prefill_body.cuh, EXP).
 //
 // The converting form of that kernel redoes the conversion for every 128-row tile, and its
-// converters' 3000 instructions a key tile share the SM with the softmax (913 us for four
-// ragged chunks of 300..2048 rows, 32/8 heads; 805 us in this form, 649 us from a 16-bit pool).  Expanding costs
-// 512 bytes of writes per token and kv head, once.  It is used from four row tiles on, while
+// converters' 3000 instructions a key tile share the SM with the softmax: 913 us for four ragged
+// chunks of 300..2048 rows (32/8 heads), 805 us in this form, 649 us from a 16-bit pool.  It costs
+// 512 bytes of writes per token and kv head, once, and is used from four row tiles on, while
 // the expanded copy (bounded by the tables' width) stays below SCRATCH_MAX.
 
 #include <algorithm>
