@@ -455,7 +455,8 @@ def score_mods(device: torch.device, num_q_heads: int, num_seqs: int, softcap: f
         if t.device != device or t.dtype != dt or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{name} must be {n} contiguous {dt} values on {device}, got "
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return L.ScoreMods(float(softcap), int(window), _ptr(alibi_slopes), _ptr(prefix_lens))
+    # (int32 on the other side; a wider window hides nothing either)
+    return L.ScoreMods(float(softcap), min(int(window), 2 ** 31 - 1), _ptr(alibi_slopes), _ptr(prefix_lens))
 
 
 _stream_workspaces: Dict[Tuple[int, int], torch.Tensor] = {}

@@ -219,7 +219,8 @@ static int to_scored(const mf_attention_args* args, const mf_score_mods* mods, i
   if (!mods) return fail(MF_EINVAL, "scored attention: null mods");
   if (!(mods->softcap >= 0.f) || mods->softcap > 1e30f || mods->window < 0)
     return fail(MF_EINVAL, "scored attention: softcap and window must not be negative");
-  p.mods = {mods->softcap, mods->alibi_slopes, mods->window, mods->prefix_lens};
+  p.mods = {mods->softcap, mods->alibi_slopes, bounded_window(mods->window, p.max_q_len),
+            mods->prefix_lens};
   if (p.mods.any() && (p.wk || p.n_peers > 0))
     return fail(MF_EUNSUPPORTED, "scored attention: a side window or peer output is not served "
                                  "with score modifiers");

@@ -20,6 +20,12 @@ struct ScoreMods {
   }
 };
 
+// A window that reaches back behind every row's position (rows start at max_q_len - 1 before the
+// first key at the earliest) hides nothing; bounded so that p - window + 1 stays in 32 bits.
+inline int32_t bounded_window(int32_t window, int32_t max_q_len) {
+  return window < INT32_MAX - max_q_len ? window : INT32_MAX - max_q_len;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 MF_DEVINL float rcp_approx(float x) {

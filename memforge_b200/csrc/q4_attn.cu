@@ -1094,7 +1094,8 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
   P.a.scale = a->scale;
   P.a.causal = a->causal;
   P.a.err = err;
-  P.a.mods = {a->mods.softcap, a->mods.alibi_slopes, a->mods.window, a->mods.prefix_lens};
+  P.a.mods = {a->mods.softcap, a->mods.alibi_slopes,
+              bounded_window(a->mods.window, P.a.max_q_len), a->mods.prefix_lens};
   P.G = a->num_q_heads / a->num_kv_heads;
   P.g_mul = (uint32_t)(((1ull << 32) + P.G - 1) / P.G);
   if (P.G > 255 || (int64_t)P.a.max_q_len * P.G >= (1 << 24))

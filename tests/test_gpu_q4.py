@@ -577,3 +577,11 @@ def test_many_row_tiles_non_causal_without_keys_and_extremes(wide):
 def test_many_row_tiles_of_every_group_size():
     for hq, hkv, ql in ((4, 4, 700), (28, 4, 100), (8, 4, 300), (80, 5, 40), (96, 2, 60)):
         Case(67 + hq, "bf16", hq, hkv, 128, [ql + 5, ql + 300, ql], [ql] * 3).check()
+
+
+@pytest.mark.parametrize("hq,hkv,kv,ql", [(8, 2, [3, 90], 6), (32, 8, [100, 700], 300),
+                                          (32, 8, [20, 400], 60)])
+def test_the_widest_window_hides_nothing(hq, hkv, kv, ql):
+    c = Case(60, "bf16", hq, hkv, 128, kv, [ql] * 2, window=2 ** 31 - 1)
+    got = c.check()
+    assert (c.run(window=1 << 20).double().cpu().numpy() == got).all()

@@ -223,3 +223,10 @@ def test_bad_tables_are_reported():
     c.run()
     with pytest.raises(IndexError, match="block table entry"):
         K.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,d,ql", [("bf16", 128, 2), ("bf16", 128, 200), ("f32", 80, 6)])
+def test_the_widest_window_hides_nothing(dtype, d, ql):
+    c = Case(40, dtype, 8, 2, d, [max(ql // 2, 1), 3 * ql + 40], [ql] * 2, window=2 ** 31 - 1)
+    got = c.check()
+    assert (c.run(window=1 << 20) == torch.from_numpy(got).cuda().to(TORCH_DT[dtype])).all()

@@ -138,6 +138,11 @@ def test_modifier_values_are_refused():
             K.score_mods(cpu, 4, 2, **v)
 
 
+def test_a_window_past_32_bits_is_no_narrow_one():
+    cpu = torch.device("cpu")
+    assert K.score_mods(cpu, 4, 2, 0.0, 2 ** 32 + 5, None, None).window == 2 ** 31 - 1
+
+
 def test_pool_shapes_are_refused():
     for t in (torch.zeros((2, 2, 2176)), torch.zeros((2, 2, 2000), dtype=torch.uint8),
               torch.zeros((2, 2, 1408), dtype=torch.uint8), torch.zeros((2, 2176), dtype=torch.uint8),
