@@ -377,8 +377,8 @@ MF_API int mf_accept_commit(const mf_accept_args* args, mf_stream_t stream);
  *                      ((not causal or k <= p) and (window == 0 or p - k < window)))
  * where row i of a sequence is at p = kv_len - q_len + i.  A prefix is seen by every
  * row, earlier ones included, and stays visible behind a window.  A row that sees no key is
- * written as zeros.  A zero / NULL member leaves its step out; softcap and window
- * must not be negative.
+ * written as zeros.  A zero / NULL member leaves its step out (all of them: the call is
+ * mf_paged_attention); softcap is 0 or from 1e-30 to 1e30, window not negative.
  */
 typedef struct {
   float softcap;

@@ -444,8 +444,8 @@ def score_mods(device: torch.device, num_q_heads: int, num_seqs: int, softcap: f
     """The checked ``mf_score_mods``, or None when no modifier is given."""
     if not softcap and not window and alibi_slopes is None and prefix_lens is None:
         return None
-    if not 0.0 <= softcap <= 1e30:
-        raise ValueError(f"softcap must be 0 (none) or positive, got {softcap}")
+    if softcap != 0.0 and not 1e-30 <= softcap <= 1e30:
+        raise ValueError(f"softcap must be 0 (none) or from 1e-30 to 1e30, got {softcap}")
     if window < 0:
         raise ValueError(f"window must be 0 (none) or positive, got {window}")
     for name, t, dt, n in (("alibi_slopes", alibi_slopes, torch.float32, num_q_heads),

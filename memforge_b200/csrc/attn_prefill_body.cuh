@@ -46,7 +46,7 @@
 // out, and so are the pages of a tile that lie behind the window.  The cap is a
 // polynomial while a warp's scores stay below 3/4 of it (3.5 packed instructions per
 // score, where the exponential and the reciprocal would add two SFU operations to the
-// softmax's one), else softcap_log2.
+// softmax's one), else softcap_large_log2.
 //
 // Every mbarrier wait is bounded; on expiry the CTA raises MF_ERR_TIMEOUT, drains
 // its TMA loads and MMAs, frees its TMEM and returns.
@@ -294,7 +294,7 @@ MF_DEVINL void cap_scores(float* sv, float sl2, float cap2) {
     const float two_over = 2.f / cap2;
 #pragma unroll
     for (int c = 0; c < N; ++c)  // exp(2 s / cap) = 2^(2 log2(e) s2 / cap2)
-      sv[c] = softcap_log2(sv[c] * sl2, cap2, two_over * kLog2e);
+      sv[c] = softcap_large_log2(sv[c] * sl2, cap2, two_over * kLog2e);
   } else {
     const uint64_t k2 = f32x2(ky, ky), s2 = f32x2(cap2, cap2);
     const uint64_t c0 = f32x2(CAP2[0], CAP2[0]), c1 = f32x2(CAP2[1], CAP2[1]),

@@ -217,8 +217,9 @@ static int to_scored(const mf_attention_args* args, const mf_score_mods* mods, i
   const int rc = to_params(args, err, p);
   if (rc != MF_OK) return rc;
   if (!mods) return fail(MF_EINVAL, "scored attention: null mods");
-  if (!(mods->softcap >= 0.f) || mods->softcap > 1e30f || mods->window < 0)
-    return fail(MF_EINVAL, "scored attention: softcap and window must not be negative");
+  if (!softcap_ok(mods->softcap) || mods->window < 0)
+    return fail(MF_EINVAL, "scored attention: softcap must be 0 or from 1e-30 to 1e30, window not "
+                           "negative");
   p.mods = {mods->softcap, mods->alibi_slopes, bounded_window(mods->window, p.max_q_len),
             mods->prefix_lens};
   if (p.mods.any() && (p.wk || p.n_peers > 0))

@@ -20,6 +20,9 @@ struct ScoreMods {
   }
 };
 
+// (a smaller cap's reciprocal is not finite in fp32; a NaN fails both)
+inline bool softcap_ok(float cap) { return cap == 0.f || (cap >= 1e-30f && cap <= 1e30f); }
+
 // A window that reaches back behind every row's position (rows start at max_q_len - 1 before the
 // first key at the earliest) hides nothing; bounded so that p - window + 1 stays in 32 bits.
 inline int32_t bounded_window(int32_t window, int32_t max_q_len) {
@@ -39,8 +42,18 @@ MF_DEVINL float rcp_approx(float x) {
 // From tanh(y) = 1 - 2 / (1 + exp(2y)): absolute error about cap2 * 2^-23, where the
 // hardware's own tanh (relative 2^-11) would move a weight by cap * 2^-11.  An
 // overflowing exponential gives rcp(inf) = 0, the cap itself.
-MF_DEVINL float softcap_log2(float s2, float cap2, float two_over) {
+MF_DEVINL float softcap_large_log2(float s2, float cap2, float two_over) {
   return fmaf(-2.f * cap2, rcp_approx(1.f + fast_exp2(s2 * two_over)), cap2);
+}
+
+// The same, and below a quarter of the cap its series (relative error 4e-7), so that the
+// error stays within |s2| * 2^-21 however large the cap is.
+MF_DEVINL float softcap_log2(float s2, float cap2, float two_over) {
+  constexpr float H2 = 0.34657359f * 0.34657359f;  // (ln 2 / 2)^2: y = z ln 2 / 2
+  const float z = s2 * two_over, u = z * z;
+  const float t = fmaf(u, fmaf(u, fmaf(u, -17.f / 315.f * H2 * H2 * H2, 2.f / 15.f * H2 * H2),
+                               -1.f / 3.f * H2), 1.f);
+  return fabsf(z) < 0.72f ? s2 * t : softcap_large_log2(s2, cap2, two_over);
 }
 
 }  // namespace mf

@@ -1064,8 +1064,9 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
   if (a->num_seqs > 0 && a->total_q > 0 &&
       (!a->q || !a->out || !a->pool || !a->block_tables || !a->kv_lens))
     return fail(MF_EINVAL, "q4 attention: null pointer");
-  if (!(a->mods.softcap >= 0.f) || a->mods.softcap > 1e30f || a->mods.window < 0)
-    return fail(MF_EINVAL, "q4 attention: softcap and window must not be negative");
+  if (!softcap_ok(a->mods.softcap) || a->mods.window < 0)
+    return fail(MF_EINVAL, "q4 attention: softcap must be 0 or from 1e-30 to 1e30, window not "
+                           "negative");
   P = q4a::Params{};
   P.a.q = a->q;
   P.a.q_sr = a->q_stride_row;

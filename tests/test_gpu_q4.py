@@ -585,3 +585,19 @@ def test_the_widest_window_hides_nothing(hq, hkv, kv, ql):
     c = Case(60, "bf16", hq, hkv, 128, kv, [ql] * 2, window=2 ** 31 - 1)
     got = c.check()
     assert (c.run(window=1 << 20).double().cpu().numpy() == got).all()
+
+
+@pytest.mark.parametrize("softcap", [1e-30, 1e-3, 1e5, 1e7, 1e30])
+@pytest.mark.parametrize("dtype,ql", [("bf16", 1), ("f32", 3)])
+def test_caps_far_from_the_scores(softcap, dtype, ql):
+    # Beyond the scores a cap leaves them as they are: its error scales with the scores
+    # (at most 4 * 2^-21 of the largest), not with the cap.
+    c = Case(61, dtype, 8, 2, 128, [90, 300], [ql] * 2, softcap=softcap)
+    want, tol = c.want()
+    slots = (c.tables[..., None] * 16 + np.arange(16)).reshape(-1)
+    k, v = R.read_rows(c.pool, 128, slots[slots >= 0])
+    size = c.scale * np.abs(c.q).sum(-1, keepdims=True) * np.nanmax(np.abs(k))
+    tol = tol + 4 * 4 * 2.0 ** -21 * np.minimum(size, softcap) * np.nanmax(np.abs(v))
+    got = c.run().double().cpu().numpy()
+    K.check_device_errors()
+    assert (np.abs(got - want) <= tol).all()

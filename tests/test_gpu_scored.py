@@ -230,3 +230,21 @@ def test_the_widest_window_hides_nothing(dtype, d, ql):
     c = Case(40, dtype, 8, 2, d, [max(ql // 2, 1), 3 * ql + 40], [ql] * 2, window=2 ** 31 - 1)
     got = c.check()
     assert (c.run(window=1 << 20) == torch.from_numpy(got).cuda().to(TORCH_DT[dtype])).all()
+
+
+@pytest.mark.parametrize("softcap", [1e-30, 1e-3, 1e5, 1e7, 1e30])
+@pytest.mark.parametrize("dtype,d,ql", [("bf16", 128, 1), ("bf16", 128, 60), ("f32", 80, 2)])
+def test_caps_far_from_the_scores(softcap, dtype, d, ql):
+    # Beyond the scores a cap leaves them as they are: its error scales with the scores
+    # (at most 4 * 2^-21 of the largest), not with the cap; below them, with the cap.
+    c = Case(41, dtype, 8, 2, d, [90, 300], [ql] * 2, softcap=softcap)
+    want, tol = c.want()
+    if softcap > 1:
+        c.softcap = 0.0
+        tol = c.want()[1]
+        size = c.scale * np.abs(c.q).sum(-1, keepdims=True) * np.abs(c.k).max()
+        tol = tol + 4 * 4 * 2.0 ** -21 * size * np.abs(c.v).max()
+        c.softcap = softcap
+    got = c.run().double().cpu().numpy()
+    K.check_device_errors()
+    assert (np.abs(got - want) <= tol).all()

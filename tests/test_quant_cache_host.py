@@ -138,6 +138,13 @@ def test_modifier_values_are_refused():
             K.score_mods(cpu, 4, 2, **v)
 
 
+@pytest.mark.parametrize("cap", [1e-38, 1e31, float("inf")])
+def test_caps_outside_the_range_are_refused(cap):
+    with pytest.raises(ValueError, match="softcap"):
+        K.score_mods(torch.device("cpu"), 4, 2, cap, 0, None, None)
+    assert L.lib().mf_q4_paged_attention(args(softcap=cap), None, 0, None, None) == L.MF_EINVAL
+
+
 def test_a_window_past_32_bits_is_no_narrow_one():
     cpu = torch.device("cpu")
     assert K.score_mods(cpu, 4, 2, 0.0, 2 ** 32 + 5, None, None).window == 2 ** 31 - 1
