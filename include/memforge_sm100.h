@@ -378,7 +378,8 @@ MF_API int mf_accept_commit(const mf_accept_args* args, mf_stream_t stream);
  * where row i of a sequence is at p = kv_len - q_len + i.  A prefix is seen by every
  * row, earlier ones included, and stays visible behind a window.  A row that sees no key is
  * written as zeros.  A zero / NULL member leaves its step out (all of them: the call is
- * mf_paged_attention); softcap is 0 or from 1e-30 to 1e30, window not negative.
+ * mf_paged_attention); softcap is 0 or from 1e-30 to 1e30, window not negative, scale from
+ * 1e-9 to 1e9.
  */
 typedef struct {
   float softcap;
@@ -448,7 +449,8 @@ MF_API int mf_q4_gather_kv(const void* pool, int64_t pool_stride_block, int64_t 
 /*
  * Attention over a 4-bit pool: rows, tables, lengths and masks as in
  * mf_paged_attention (q_per_seq or cu_seqlens_q; decode, verify and chunks), q and
- * out of `dtype`, with the score modifiers of `mods` (all zero: none).  Every row of
+ * out of `dtype`, with the score modifiers of `mods` (all zero: none) and a scale from
+ * 1e-9 to 1e9.  Every row of
  * the run is read from the pool: write the step's keys first.  A row without a
  * visible key (kv_len 0, or kv_len < q_len) is written as zeros, without an error.
  * A negative kv_len or a run longer than max_q_len sets MF_ERR_LENGTH, a table too short

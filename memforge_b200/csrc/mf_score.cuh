@@ -20,6 +20,10 @@ struct ScoreMods {
   }
 };
 
+// Kernels take maxima of unscaled scores and mask those with -inf, which a negative or
+// vanishing scale would turn into the largest.  (A NaN fails.)
+inline bool scale_ok(float scale) { return scale >= 1e-9f && scale <= 1e9f; }
+
 // (a smaller cap's reciprocal is not finite in fp32; a NaN fails both)
 inline bool softcap_ok(float cap) { return cap == 0.f || (cap >= 1e-30f && cap <= 1e30f); }
 

@@ -1067,6 +1067,8 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
   if (!softcap_ok(a->mods.softcap) || a->mods.window < 0)
     return fail(MF_EINVAL, "q4 attention: softcap must be 0 or from 1e-30 to 1e30, window not "
                            "negative");
+  if (!scale_ok(a->scale))
+    return fail(MF_EINVAL, "q4 attention: scale must be from 1e-9 to 1e9");
   P = q4a::Params{};
   P.a.q = a->q;
   P.a.q_sr = a->q_stride_row;
