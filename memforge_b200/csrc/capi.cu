@@ -225,6 +225,9 @@ static int to_scored(const mf_attention_args* args, const mf_score_mods* mods, i
   if (p.mods.any() && (p.wk || p.n_peers > 0))
     return fail(MF_EUNSUPPORTED, "scored attention: a side window or peer output is not served "
                                  "with score modifiers");
+  if (p.mods.any() && !p.cu_q && p.total_q > 0 &&
+      (int64_t)p.num_seqs * p.q_per_seq > p.total_q)
+    return fail(MF_EINVAL, "scored attention: total_q below num_seqs * q_per_seq");
   if (p.mods.any() && !scale_ok(p.scale))
     return fail(MF_EINVAL, "scored attention: scale must be from 1e-9 to 1e9");
   return MF_OK;

@@ -1067,6 +1067,8 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
   if (!softcap_ok(a->mods.softcap) || a->mods.window < 0)
     return fail(MF_EINVAL, "q4 attention: softcap must be 0 or from 1e-30 to 1e30, window not "
                            "negative");
+  if (!a->cu_seqlens_q && a->total_q > 0 && (int64_t)a->num_seqs * a->q_per_seq > a->total_q)
+    return fail(MF_EINVAL, "q4 attention: total_q below num_seqs * q_per_seq");
   if (!scale_ok(a->scale))
     return fail(MF_EINVAL, "q4 attention: scale must be from 1e-9 to 1e9");
   P = q4a::Params{};
@@ -1114,7 +1116,7 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
 Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
   Plan pl{};
   int64_t rows = (int64_t)P.a.max_q_len * P.G;
-  pl.chunks = chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
+  pl.chunks = P.width > 0 && chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
   pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
   pl.expand = pl.chunks && q4_expand_plan(P.a, P.width, P.vec, dt, pl.scratch);
   if (!pl.tiles) {

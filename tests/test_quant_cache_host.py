@@ -159,6 +159,19 @@ def test_scales_that_order_nothing_are_refused(scale):
                                              None) == L.MF_EINVAL
 
 
+def test_fewer_rows_than_the_sequences_have_are_refused():
+    bad = args(q_per_seq=3, total_q=5)
+    assert L.lib().mf_q4_paged_attention(bad, None, 0, None, None) == L.MF_EINVAL
+    a = L.AttentionArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.q = a.out = a.k_pool = a.v_pool = a.block_tables = a.kv_lens = 0x1000
+    a.num_blocks, a.block_size, a.table_stride = 4, 16, 4
+    a.q_per_seq, a.num_seqs, a.total_q, a.max_q_len = 2, 2, 3, 2
+    a.num_q_heads, a.num_kv_heads, a.head_dim, a.dtype, a.scale = 2, 2, 128, L.MF_BF16, 0.1
+    assert L.lib().mf_paged_attention_scored(a, L.ScoreMods(9.0, 0, None, None), None, 0, None,
+                                             None) == L.MF_EINVAL
+
+
 def test_a_window_past_32_bits_is_no_narrow_one():
     cpu = torch.device("cpu")
     assert K.score_mods(cpu, 4, 2, 0.0, 2 ** 32 + 5, None, None).window == 2 ** 31 - 1
