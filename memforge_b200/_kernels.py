@@ -86,9 +86,16 @@ def check_device_errors(device: Optional[torch.device] = None, reset: bool = Tru
     bits = int(w.item())
     if reset and bits:
         w.zero_()
-        ws = _workspaces.get(device.index if device.index is not None else torch.cuda.current_device())
-        if ws is not None:
+        idx = device.index if device.index is not None else torch.cuda.current_device()
+        left = [ws for key, ws in list(_stream_workspaces.items()) if key[0] == idx]
+        if left:
+            torch.cuda.synchronize(device)   # other streams' launches may be using theirs
+        if idx in _workspaces:
+            left.append(_workspaces[idx])
+        for ws in left:
             ws.zero_()   # an aborted launch may leave arrival counters behind
+        if len(left) > 1:
+            torch.cuda.synchronize(device)
     if bits:
         raise IndexError(f"memforge_b200 kernel reported: {L.describe_err(bits)} (0x{bits:x})")
 

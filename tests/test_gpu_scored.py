@@ -248,3 +248,14 @@ def test_caps_far_from_the_scores(softcap, dtype, d, ql):
     got = c.run().double().cpu().numpy()
     K.check_device_errors()
     assert (np.abs(got - want) <= tol).all()
+
+
+def test_an_aborted_launch_leaves_no_counters_behind():
+    c = Case(42, "bf16", 8, 2, 128, [4000, 33], [1, 1], window=500)
+    c.check()
+    ws = K._stream_workspaces[(0, torch.cuda.current_stream().cuda_stream)]
+    ws[:64] = 7   # as a launch that gave up in mid-way would leave them
+    K.err_word(torch.device("cuda", 0)).fill_(1)
+    with pytest.raises(IndexError):
+        K.check_device_errors()
+    c.check()
