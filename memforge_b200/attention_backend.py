@@ -294,7 +294,8 @@ def _unbound(module, query, key, value, attention_mask, scale, out, mods):
     Hkv, kv_len = key.shape[1], key.shape[2]
     causal = bool(getattr(module, "is_causal", True))
     if attention_mask is not None:
-        _require_plain(attention_mask, q_len, kv_len, causal)
+        mods = dict(mods, window=_require_plain(attention_mask, q_len, kv_len, causal,
+                                                mods.get("window", 0)))
     bs = 16
     nblk = (kv_len + bs - 1) // bs
     pool_k = torch.zeros((B * nblk, bs, Hkv, D), dtype=query.dtype, device=query.device)
@@ -311,8 +312,12 @@ def _unbound(module, query, key, value, attention_mask, scale, out, mods):
     return out
 
 
-def _require_plain(mask: torch.Tensor, q_len: int, kv_len: int, causal: bool) -> None:
-    """Accept only the mask the kernel computes itself (bottom-right causal, or none)."""
+def _require_plain(mask: torch.Tensor, q_len: int, kv_len: int, causal: bool,
+                   window: int = 0) -> int:
+    """
+    Accept only a mask the kernel computes itself: bottom-right causal or none, or either
+    with the call's window.  Returns the window that the mask has (0: none).
+    """
     allowed = mask if mask.dtype == torch.bool else (mask == 0)
     allowed = allowed[..., :kv_len]
     if causal:
@@ -320,7 +325,11 @@ def _require_plain(mask: torch.Tensor, q_len: int, kv_len: int, causal: bool) ->
         want = torch.arange(kv_len, device=mask.device)[None, :] <= rows
     else:
         want = torch.ones((q_len, kv_len), dtype=torch.bool, device=mask.device)
-    if not bool((allowed == want).all()):
+    if bool((allowed == want).all()):
+        return 0
+    rows = torch.arange(q_len, device=mask.device)[:, None] + (kv_len - q_len)
+    near = rows - torch.arange(kv_len, device=mask.device)[None, :] < window
+    if not window or not bool((allowed == (want & near)).all()):
         raise NotImplementedError(
             "memforge_paged: this attention mask (padding or a custom pattern) is not "
             "expressible by the paged kernel; bind a paged cache or pack the batch "

@@ -194,3 +194,18 @@ def test_pool_accounting():
     assert pool.describe()["bytes_per_token"] == 3 * 2 * 136
     with pytest.raises(ValueError, match="16 tokens"):
         Q.Q4KVPool(spec, 5, block_size=32)
+
+
+def test_a_mask_handed_to_the_attention_function_decides_about_its_window():
+    from memforge_b200 import attention_backend as AB
+    p, k = torch.arange(3)[:, None] + 4, torch.arange(7)[None]
+    causal, near = k <= p, p - k < 3
+    as_bias = torch.where(causal & near, 0.0, float("-inf"))
+    assert AB._require_plain(causal, 3, 7, True) == 0
+    assert AB._require_plain(causal, 3, 7, True, 3) == 0      # the mask has no window
+    assert AB._require_plain(causal & near, 3, 7, True, 3) == 3
+    assert AB._require_plain(as_bias[None, None], 3, 7, True, 3) == 3
+    assert AB._require_plain(near, 3, 7, False, 3) == 3
+    for window, mask in ((0, causal & near), (2, causal & near), (3, causal & (k != 2))):
+        with pytest.raises(NotImplementedError):
+            AB._require_plain(mask, 3, 7, True, window)
