@@ -334,6 +334,7 @@ def _require_plain(mask: torch.Tensor, q_len: int, kv_len: int, causal: bool,
             "memforge_paged: this attention mask (padding or a custom pattern) is not "
             "expressible by the paged kernel; bind a paged cache or pack the batch "
             "(varlen_attention_context) instead")
+    return window
 
 
 def paged_mask(batch_size: int, q_length: int, kv_length: int, q_offset: int = 0,
