@@ -4,9 +4,12 @@
 //
 // The converting form of that kernel redoes the conversion for every 128-row tile, and its
 // converters' 3000 instructions a key tile share the SM with the softmax: 913 us for four ragged
-// chunks of 300..2048 rows (32/8 heads), 805 us in this form, 649 us from a 16-bit pool.  It costs
-// 512 bytes of writes per token and kv head, once, and is used from four row tiles on, while
-// the expanded copy (bounded by the tables' width) stays below SCRATCH_MAX.
+// chunks of 300..2048 rows (32/8 heads), 665 us in this form, 649 us from a 16-bit pool.  It costs
+// 512 bytes of writes per token and kv head, once, and is used from six row tiles of a kv head
+// on, while the expanded copy (bounded by the tables' width) stays below SCRATCH_MAX.  Against
+// converting, 16 sequences of 2000 / 8000 keys, 8 kv heads: four tiles 114 : 116 / 393 : 331 us,
+// six 149 : 167 / 510 : 487, eight 176 : 199 / 605 : 607, sixteen 293 : 370 / 1038 : 1185; four
+// sequences, six tiles: 50 : 59 / 150 : 159.
 
 #include <algorithm>
 
@@ -18,7 +21,7 @@ namespace mf {
 namespace pf {
 
 constexpr size_t SCRATCH_MAX = size_t(1) << 30;
-constexpr int MIN_ROWS = 4 * BM;
+constexpr int MIN_ROWS = 6 * BM;
 
 template <typename T, bool MOD>
 __global__ void __launch_bounds__(THREADS, 1) q4_expanded_kernel(

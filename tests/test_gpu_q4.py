@@ -601,3 +601,21 @@ def test_caps_far_from_the_scores(softcap, dtype, ql):
     got = c.run().double().cpu().numpy()
     K.check_device_errors()
     assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("hq,hkv,ql", [(4, 4, 800), (28, 4, 120), (8, 4, 400), (80, 5, 56),
+                                       (9, 3, 300)])
+def test_runs_of_six_row_tiles_of_every_group_size(hq, hkv, ql):
+    Case(70 + hq, "bf16", hq, hkv, 128, [ql + 5, ql + 300, ql], [ql] * 3).check()
+
+
+def test_runs_of_six_row_tiles_non_causal_without_keys_and_extremes():
+    Case(71, "bf16", 16, 4, 128, [250, 9, 400], [220] * 3, causal=False).check()
+    got = Case(72, "bf16", 16, 4, 128, [0, 20, 300], [200] * 3).check()
+    assert not got[:200].any() and not got[200:380].any() and got[380:400].any()
+    c = Case(73, "bf16", 16, 4, 128, [250, 200, 230], [200] * 3, q_scale=1e-6)
+    par = c.pool[:, :, 16 * 128:].view(np.float16).reshape(-1, 4, 2, 16, 2)
+    par[:, :, :, 0::3] = (8728.0, -65504.0)   # codes reach 65416
+    par[:, :, :, 1::3] = (0.5, 60000.0)
+    par[:, :, :, 2::3] = (2.0 ** -24, -2.0 ** -20)
+    c.check()
