@@ -189,6 +189,16 @@ struct Params {
   int width;         // Q4, EXP: entries of a block table's row
   int vec;           // Q4: q and out rows allow 16-byte accesses
   const float* qs;   // EXP: per (row, query head), what scales S to log2 units
+  float cap2, inv_cap2, two_over;  // softcap in log2 units, its inverse, 2 / softcap: divided
+                                   // on the host, where it costs the tile loop no registers
+
+  // The scale and the cap of the call.
+  void set_scores() {
+    scale_log2 = a.scale * kLog2e;
+    cap2 = a.mods.softcap * kLog2e;
+    inv_cap2 = a.mods.softcap > 0.f ? 1.f / cap2 : 0.f;
+    two_over = a.mods.softcap > 0.f ? 2.f / a.mods.softcap : 0.f;
+  }
 };
 
 // Geometry of one work item (identical in every role).
@@ -278,8 +288,8 @@ constexpr float CAP2[5] = {0.9999972283095431f, -0.33323076454511924f, 0.1322609
 // factors take in sl2 and the cap, so the short one is four packed operations a pair; the
 // largest score of the warp's rows decides.
 template <int N>
-MF_DEVINL void cap_scores(float* sv, float sl2, float cap2) {
-  const float ky = sl2 / cap2;
+MF_DEVINL void cap_scores(const Params& P, float* sv, float sl2) {
+  const float ky = sl2 * P.inv_cap2;
   float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < N; c += 2)
@@ -295,12 +305,11 @@ MF_DEVINL void cap_scores(float* sv, float sl2, float cap2) {
       f32x2_split(f32x2_mul(v, f32x2_fma(u, f32x2_fma(u, c2, c1), c0)), sv[c], sv[c + 1]);
     }
   } else if (__any_sync(0xffffffffu, mx > CAP_MAX2)) {
-    const float two_over = 2.f / cap2;
 #pragma unroll
     for (int c = 0; c < N; ++c)  // exp(2 s / cap) = 2^(2 log2(e) s2 / cap2)
-      sv[c] = softcap_large_log2(sv[c] * sl2, cap2, two_over * kLog2e);
+      sv[c] = softcap_large_log2(sv[c] * sl2, P.cap2, P.two_over);
   } else {
-    const uint64_t k2 = f32x2(ky, ky), s2 = f32x2(cap2, cap2);
+    const uint64_t k2 = f32x2(ky, ky), s2 = f32x2(P.cap2, P.cap2);
     const uint64_t c0 = f32x2(CAP2[0], CAP2[0]), c1 = f32x2(CAP2[1], CAP2[1]),
                    c2 = f32x2(CAP2[2], CAP2[2]), c3 = f32x2(CAP2[3], CAP2[3]),
                    c4 = f32x2(CAP2[4], CAP2[4]);
@@ -951,7 +960,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
         const int kbase = I.template tile<MOD>(j) * BN;
         const int lim = win_tile ? pos : limit - kbase;
         if constexpr (MOD) {
-          if (P.a.mods.softcap > 0.f) cap_scores<CW>(sv, raw_sl2, P.a.mods.softcap * kLog2e);
+          if (P.a.mods.softcap > 0.f) cap_scores<CW>(P, sv, raw_sl2);
           if (P.a.mods.slopes) {
             const float up = P.a.mods.softcap > 0.f ? 1.f : raw_sl2;
             const uint64_t up2 = f32x2(up, up), two = f32x2(2.f * slope, 2.f * slope);

@@ -79,7 +79,7 @@ int launch_attn_prefill_tc(const AttnParams& p, mf_dtype dtype, int rows_cap,
   P.a = p;
   P.G = G;
   P.rows_cap = rows_cap;
-  P.scale_log2 = p.scale * 1.4426950408889634f;
+  P.set_scores();
   P.in_fmt = dtype == MF_BF16 ? 1u : 0u;
   P.window = p.wk ? 1 : 0;
   // Persistent grid: one CTA per SM, or fewer when there are fewer items

@@ -204,7 +204,7 @@ int launch_q4_expanded(const AttnParams& a, int width, int rows_cap, const Q4Scr
   P.a = a;
   P.G = a.hq / a.hkv;
   P.rows_cap = rows_cap;
-  P.scale_log2 = a.scale * kLog2e;
+  P.set_scores();
   P.in_fmt = 0;  // fp16 operands
   P.width = width;
   P.vec = 1;

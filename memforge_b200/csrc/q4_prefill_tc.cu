@@ -66,7 +66,7 @@ int launch_q4_prefill(const AttnParams& a, int width, int vec, int rows_cap,
   P.a = a;
   P.G = a.hq / a.hkv;
   P.rows_cap = rows_cap;
-  P.scale_log2 = a.scale * kLog2e;
+  P.set_scores();
   P.in_fmt = 0;  // fp16 operands
   P.width = width;
   P.vec = vec;
