@@ -343,6 +343,28 @@ MF_DEVINL void code_pairs(uint32_t w, uint32_t* p) {
     p[2 * i + 1] = half2_fma((v & 0x00F000F0u) | K1024, SIXTEENTH, M64);
   }
 }
+MF_DEVINL uint32_t half2_max(uint32_t a, uint32_t b) {  // (a NaN is passed over)
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Whether 15 * scale + base can pass fp16's largest number, of (scale, base) or the largest of
+// several; such values are then held to that number.  Only a row that reaches it has them:
+// scale's rounding up takes its largest code at most 120 past its largest value.
+MF_DEVINL bool past_range(uint32_t params) {
+  const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&params));
+  return fmaf(15.f, p.x, p.y) > 65504.f;
+}
+MF_DEVINL uint32_t held(uint32_t v) {
+  asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7BFF7BFFu));
+  return v;
+}
+MF_DEVINL void lds128(uint32_t addr, uint32_t* v) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
 MF_DEVINL void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
                "r"(d)
@@ -451,10 +473,7 @@ MF_DEVINL void q4_stage_q(const Params& P, const Item& I, uint32_t tile, float* 
     const int r = q4_q_row(it, ts);
     const uint32_t dst = chunk_at(tile, r, c);
     uint32_t raw[4];
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3])
-                 : "r"(dst)
-                 : "memory");
+    lds128(dst, raw);
     const T* t = reinterpret_cast<const T*>(raw);
     float x[8];
 #pragma unroll
@@ -466,7 +485,7 @@ MF_DEVINL void q4_stage_q(const Params& P, const Item& I, uint32_t tile, float* 
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int ex = (int)(__float_as_uint(top) >> 23);
     const float mul = __uint_as_float((uint32_t)min(max(268 - ex, 1), 240) << 23);
-    if (c == 0) qs[r] = 2.f * P.scale_log2 / mul;
+    if (c == 0) qs[r] = P.scale_log2 / mul;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= mul;
     sts128(dst, Mma<__half>::pack(x[0], x[4]), Mma<__half>::pack(x[1], x[5]),
@@ -476,10 +495,10 @@ MF_DEVINL void q4_stage_q(const Params& P, const Item& I, uint32_t tile, float* 
 
 // K or V of every tile, by four warps; ts: thread of the 128, which take the pages of a tile
 // two at a time.  The K warps bring an item's Q after its first K tile.  Codes become
-// n * scale + base halved, in fp16 (one rounding; halved so that no code of a row passes fp16's
-// range; the scores and the output take the factor back), stored as the swizzled tile the MMA
-// reads.  Keys without a token (or behind every row's window) become zeros, whatever their
-// slots hold.  K's dims stay in the order the masks give inside each group of eight
+// n * scale + base in fp16 with one rounding: scale and base are multiples of 2^-24, so it is off
+// by at most 2^-11 of the value, and subnormal values are exact.  They are stored as the swizzled
+// tile the MMA reads.  Keys without a token (or behind every row's window) become zeros, whatever
+// their slots hold.  K's dims stay in the order the masks give inside each group of eight
 // (0 4 1 5 2 6 3 7); q is stored in the same order.
 template <typename T, bool MOD, bool V>
 MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* order, int items,
@@ -521,6 +540,7 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
       }
       const uint32_t tile = ring + st * TILE_BYTES + first * PAGE * 128;
       const uint32_t raw = base + off_raw() + rs * RAW_BYTES + first * REC;
+      uint32_t most = 0xFC00FC00u;  // largest scale and base of this thread's rows
 #pragma unroll 1
       for (int half = 0; half < PAGES / (2 * UN); ++half) {
         uint32_t w[UN][4], pr[UN][2];
@@ -549,7 +569,7 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
             const int key = key0 + (i + first) * PAGE + e;
             uint32_t v = pr[u][e];
             if (key >= I.pool_len || (MOD && key < I.lo && key >= I.pfx)) v = 0u;
-            asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x38003800u));  // x 0.5
+            most = half2_max(most, v);
             sc[e] = __byte_perm(v, v, 0x1010);
             ba[e] = __byte_perm(v, v, 0x3232);
           }
@@ -583,6 +603,20 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
           }
         }
       }
+      // Values that may pass fp16's range, held to it apart from the loop: inside, a test and a
+      // branch for every page cost the converters 6 to 9 % (16 sequences, 8 heads, four row tiles).
+      if (past_range(most)) {
+#pragma unroll 1
+        for (int i = 0; i < PAGES; i += 2) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t dst = tile + i * PAGE * 128 + at[c];
+            uint32_t v[4];
+            lds128(dst, v);
+            sts128(dst, held(v[0]), held(v[1]), held(v[2]), held(v[3]));
+          }
+        }
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -612,7 +646,7 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
 // The kernel: Q, K and V tiles by TMA from a 16-bit pool (the five tensor maps); with Q4
 // converted by warps from a 4-bit pool (no maps); with EXP by TMA from a 4-bit pool that was
 // expanded to fp16 beforehand (sequence s's page L at s * width + L, and q with it).  In the
-// latter two products and P are fp16, keys and values halved.
+// latter two keys, values and P are fp16.
 template <typename T, bool MOD, bool Q4, bool EXP = false>
 MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv,
                             const CUtensorMap* tmwk, const CUtensorMap* tmwv, const Params& P) {
@@ -893,7 +927,7 @@ MF_DEVINL void prefill_body(const CUtensorMap* tmq, const CUtensorMap* tmk, cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[B_OFREE]);  // O may be overwritten
       if (pend_valid) {
-        const float inv = FOUR ? (l_tot == 0.f ? 0.f : 2.f / l_tot) : l_tot > 0.f ? 1.f / l_tot : 0.f;
+        const float inv = FOUR ? (l_tot == 0.f ? 0.f : 1.f / l_tot) : l_tot > 0.f ? 1.f / l_tot : 0.f;
         if (Q4 && !P.vec) {  // (EXP takes calls with 16-byte rows only)
 #pragma unroll
           for (int e = 0; e < 64; ++e) pend_row[e] = from_f32<T>(__uint_as_float(o[e]) * inv);

@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) q4_expand_q(const __grid_constant__ Param
   if (!have) return;
   const int ex = (int)(__float_as_uint(top) >> 23);
   const float mul = __uint_as_float((uint32_t)min(max(268 - ex, 1), 240) << 23);
-  if (c == 0) scale[at] = 2.f * P.scale_log2 / mul;  // the keys are halved
+  if (c == 0) scale[at] = P.scale_log2 / mul;
   uint4 v;
   v.x = Mma<__half>::pack(x[0] * mul, x[1] * mul);
   v.y = Mma<__half>::pack(x[2] * mul, x[3] * mul);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256) q4_expand_q(const __grid_constant__ Param
   reinterpret_cast<uint4*>(out)[(int64_t)at * 16 + c] = v;
 }
 
-// Keys and values, halved, in fp16 (one rounding): 64 threads a record.  Tokens behind the
+// Keys and values in fp16 (one rounding): 64 threads a record.  Tokens behind the
 // sequence's last are zeros; pages that no row sees are left out.
 __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Params P, __half* k,
                                                     __half* v) {
@@ -93,17 +93,17 @@ __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Para
   const uint4 kc = __ldg(reinterpret_cast<const uint4*>(rec) + ts);
   const uint4 vc = __ldg(reinterpret_cast<const uint4*>(rec + 8 * D) + ts);
   const int kr = ts >> 2, vr = (ts >> 5) * 8 + 2 * (ts & 3);  // K row, first of two V rows
-  auto halved = [&](int off, int row, uint32_t& sc, uint32_t& ba) {
+  auto params = [&](int off, int row, uint32_t& sc, uint32_t& ba) {
     uint32_t pr = __ldg(reinterpret_cast<const uint32_t*>(rec + 16 * D + off) + row);
     if (page * PAGE + row >= len) pr = 0u;
-    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(pr) : "r"(0x38003800u));
     sc = __byte_perm(pr, pr, 0x1010);
     ba = __byte_perm(pr, pr, 0x3232);
+    return pr;
   };
   const int64_t row0 = ((int64_t)s * P.width + page) * PAGE;
   {
     uint32_t sc, ba;
-    halved(0, kr, sc, ba);
+    const bool past = past_range(params(0, kr, sc, ba));
     uint4* dst = reinterpret_cast<uint4*>(k + ((row0 + kr) * P.a.hkv + h) * D + (ts & 3) * 32);
     const uint32_t* w = &kc.x;
 #pragma unroll
@@ -112,15 +112,19 @@ __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Para
       code_pairs(w[i], p);  // (0, 4) (1, 5) (2, 6) (3, 7)
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] = half2_fma(p[e], sc, ba);
+      if (past) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = held(p[e]);
+      }
       dst[i] = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
                           __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
     }
   }
   {
     uint32_t s0, b0, s1, b1;
-    halved(64, vr, s0, b0);
-    halved(64, vr + 1, s1, b1);
+    const uint32_t p0 = params(64, vr, s0, b0), p1 = params(64, vr + 1, s1, b1);
     const uint32_t sc = __byte_perm(s0, s1, 0x5410), ba = __byte_perm(b0, b1, 0x5410);
+    const bool past = past_range(half2_max(p0, p1));
     uint4* d0 = reinterpret_cast<uint4*>(v + ((row0 + vr) * P.a.hkv + h) * D + ((ts & 31) >> 2) * 16);
     uint4* d1 = d0 + P.a.hkv * (D / 8);
     const uint32_t* w = &vc.x;
@@ -131,6 +135,10 @@ __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Para
       code_pairs(w[2 * i + 1], p + 4);
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = half2_fma(p[e], sc, ba);
+      if (past) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = held(p[e]);
+      }
       d0[i] = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
                          __byte_perm(p[4], p[5], 0x5410), __byte_perm(p[6], p[7], 0x5410));
       d1[i] = make_uint4(__byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632),

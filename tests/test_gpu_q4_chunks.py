@@ -1,0 +1,144 @@
+"""
+Long runs over the 4-bit cache on the tensor-core kernels (converting and expanded), held to
+bounds of a few percent of the output (tests/q4_bounds.py).  Every case states which of the
+two kernels it is meant for and checks that the call's plan says so.
+"""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import q4_bounds as B
+from tests import q4_reference as R
+from tests.test_gpu_q4 import as_dtype, random_pool, rng, tables_for
+
+pytestmark = pytest.mark.gpu
+
+K = pytest.importorskip("memforge_b200._kernels")
+L = pytest.importorskip("memforge_b200._lib")
+
+D = 128
+
+
+def form(num_seqs, q_per_seq, hq, hkv, width, rows):
+    """Which kernel a call of equal runs takes: the workspace tells.  Converting needs none, the
+    expanded copy takes 512 bytes a token and kv head, the mma.sync kernel its partial results."""
+    a = L.Q4AttentionArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.q = a.out = a.pool = a.block_tables = a.kv_lens = 0x1000
+    a.q_stride_row = a.out_stride_row = hq * D
+    a.q_stride_head = a.out_stride_head = D
+    a.pool_stride_block, a.pool_stride_head = hkv * 2176, 2176
+    a.num_blocks, a.table_stride, a.table_width = 4, width, width
+    a.q_per_seq, a.num_seqs, a.total_q, a.max_q_len = q_per_seq, num_seqs, rows, q_per_seq
+    a.num_q_heads, a.num_kv_heads, a.head_dim = hq, hkv, D
+    a.scale, a.causal, a.dtype = 0.1, 1, L.MF_BF16
+    need = L.lib().mf_q4_paged_attention_workspace_size(a, 0)
+    copy = 512 * num_seqs * width * 16 * hkv
+    return "converting" if need == 0 else "expanded" if need >= copy else "mma.sync"
+
+
+CONVERTING = dict(hq=16, hkv=4, kv=[200, 527, 640], ql=150)   # 60 row tiles of 16 a head, 5 of 128
+EXPANDED = dict(hq=16, hkv=4, kv=[200, 527, 640], ql=200)     # 7 of 128
+
+
+class Case:
+    def __init__(self, seed, hq, hkv, kv, ql, k_size=1.0, v_size=1.0, q_size=None, causal=True,
+                 softcap=0.0, window=0, slopes=False, prefix=None):
+        g = rng(seed)
+        self.hq, self.hkv, self.kv, self.ql = hq, hkv, list(kv), ql
+        self.causal, self.softcap, self.window = causal, softcap, window
+        self.tables, blocks = tables_for(g, kv)
+        self.pool = B.sized_pool(g, blocks, hkv, D, k_size, v_size)
+        for i, n in enumerate(kv):  # slots behind the last token: NaN parameters
+            if n % 16:
+                par = self.pool[self.tables[i, n // 16]][:, 16 * D:].reshape(hkv, 2, 16, 4)
+                par[:, :, n % 16:] = 0xFF
+                self.pool[self.tables[i, n // 16]][:, 16 * D:] = par.reshape(hkv, -1)
+        size = 1 / k_size if q_size is None else q_size
+        self.q, self.q_dev = as_dtype(g.standard_normal((len(kv) * ql, hq, D)) * size, "bf16")
+        self.slopes = (2.0 ** -(8.0 * np.arange(1, hq + 1) / hq)).astype(np.float32) if slopes else None
+        self.prefix = None if prefix is None else np.asarray(prefix, np.int32)
+        self.scale = 1 / math.sqrt(D)
+
+    def form(self):
+        return form(len(self.kv), self.ql, self.hq, self.hkv, self.tables.shape[1],
+                    len(self.kv) * self.ql)
+
+    def args(self, **kw):
+        how = dict(q_per_seq=self.ql, scale=self.scale, causal=self.causal, softcap=self.softcap,
+                   window=self.window,
+                   alibi_slopes=None if self.slopes is None else torch.from_numpy(self.slopes).cuda(),
+                   prefix_lens=None if self.prefix is None else torch.from_numpy(self.prefix).cuda())
+        how.update(kw)
+        return how
+
+    def device(self):
+        return (torch.from_numpy(self.pool).cuda(), torch.from_numpy(self.tables).cuda(),
+                torch.tensor(self.kv, dtype=torch.int32).cuda())
+
+    def run(self, q=None, out=None, **kw):
+        q = self.q_dev if q is None else q
+        out = torch.full_like(q, 7.0) if out is None else out
+        K.q4_paged_attention(q, out, *self.device(), **self.args(**kw))
+        torch.cuda.synchronize()
+        return out
+
+    def rows(self, s):
+        pos = np.arange(self.kv[s])
+        return R.read_rows(self.pool, D, self.tables[s, pos // 16] * 16 + pos % 16)
+
+    def want(self):
+        """Outputs over the operands' roundings and their bound, and by the definition."""
+        outs, tols, exact = [], [], []
+        for s, n in enumerate(self.kv):
+            q = self.q[s * self.ql:(s + 1) * self.ql]
+            k, v = self.rows(s)
+            see = R.visible(self.ql, n, self.causal, self.window,
+                            0 if self.prefix is None else int(self.prefix[s]))
+            how = (self.scale, see, self.softcap, self.slopes)
+            o, mag, size = B.attention(q, B.operand(k), B.operand(v), *how)
+            outs.append(o)
+            tols.append(B.chunk_bound("bf16", o, mag, size, n, D, self.softcap, self.slopes,
+                                      np.abs(v).max(initial=0.0)))
+            exact.append(B.attention(q, k, v, *how)[0])
+        return np.concatenate(outs), np.concatenate(tols), np.concatenate(exact)
+
+    def hold(self, got):
+        want, tol, exact = self.want()
+        assert np.isfinite(got).all()
+        err = np.abs(got - want)
+        assert (err <= tol).all(), (f"{(err > tol).mean():.2%} beyond the bound, worst "
+                                    f"{(err / tol).max():.2f} times it")
+        assert B.rms(got - exact) <= B.RMS["bf16"] * B.rms(exact)
+
+    def check(self, **kw):
+        got = self.run(**kw).double().cpu().numpy()
+        K.check_device_errors()
+        self.hold(got)
+        return got
+
+
+FORMS = [("converting", CONVERTING), ("expanded", EXPANDED)]
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 3e-5, 1e-5, 1e-6])
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_rows_of_any_size(kind, shape, size):
+    """Keys and values of one size alone in the pool; q makes up for the keys'."""
+    c = Case(80, **shape, k_size=size, v_size=size)
+    assert c.form() == kind
+    c.check()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_rows_that_reach_the_largest_fp16(kind, shape):
+    """Their largest code may stand for up to 120 more, which the kernels hold to 65504."""
+    c = Case(82, **shape, k_size=5e4, v_size=5e4)
+    assert c.form() == kind
+    k, v = c.rows(1)
+    assert (k > 65520).any() and (v > 65520).any()
+    c.check()
