@@ -355,6 +355,17 @@ MF_DEVINL bool past_range(uint32_t params) {
   const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&params));
   return fmaf(15.f, p.x, p.y) > 65504.f;
 }
+// A value row of NaN must not enter P V, where the weight 0 of a row that does not see it would
+// make a NaN of it: the value becomes zeros and its key NaN instead, and the scores, which are
+// masked row by row, carry it to the rows that see it.
+MF_DEVINL bool nan_row(uint32_t params) {  // (scale, base) not both finite
+  const uint32_t inf = 0x7C007C00u;
+  return !__hblt2(__habs2(*reinterpret_cast<const __half2*>(&params)),
+                  *reinterpret_cast<const __half2*>(&inf));
+}
+MF_DEVINL uint32_t key_params(uint32_t key, uint32_t value) {
+  return nan_row(value) ? 0x7E007E00u : key;
+}
 MF_DEVINL uint32_t held(uint32_t v) {
   asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7BFF7BFFu));
   return v;
@@ -558,7 +569,9 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
                          : "=r"(pr[u][0]), "=r"(pr[u][1])
                          : "r"(rec + par_off));
           else
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pr[u][0]) : "r"(rec + par_off));
+            asm volatile("ld.shared.u32 %0, [%2];\n\tld.shared.u32 %1, [%2 + 64];"  // K's, V's
+                         : "=r"(pr[u][0]), "=r"(pr[u][1])
+                         : "r"(rec + par_off));
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
@@ -567,7 +580,7 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
 #pragma unroll
           for (int e = 0; e < (V ? 2 : 1); ++e) {
             const int key = key0 + (i + first) * PAGE + e;
-            uint32_t v = pr[u][e];
+            uint32_t v = V ? (nan_row(pr[u][e]) ? 0u : pr[u][e]) : key_params(pr[u][0], pr[u][1]);
             if (key >= I.pool_len || (MOD && key < I.lo && key >= I.pfx)) v = 0u;
             most = half2_max(most, v);
             sc[e] = __byte_perm(v, v, 0x1010);

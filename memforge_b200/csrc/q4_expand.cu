@@ -93,8 +93,10 @@ __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Para
   const uint4 kc = __ldg(reinterpret_cast<const uint4*>(rec) + ts);
   const uint4 vc = __ldg(reinterpret_cast<const uint4*>(rec + 8 * D) + ts);
   const int kr = ts >> 2, vr = (ts >> 5) * 8 + 2 * (ts & 3);  // K row, first of two V rows
-  auto params = [&](int off, int row, uint32_t& sc, uint32_t& ba) {
-    uint32_t pr = __ldg(reinterpret_cast<const uint32_t*>(rec + 16 * D + off) + row);
+  const uint32_t* par = reinterpret_cast<const uint32_t*>(rec + 16 * D);  // K's 16, V's 16
+  auto params = [&](bool value, int row, uint32_t& sc, uint32_t& ba) {
+    const uint32_t of_v = __ldg(par + 16 + row);
+    uint32_t pr = !value ? key_params(__ldg(par + row), of_v) : nan_row(of_v) ? 0u : of_v;
     if (page * PAGE + row >= len) pr = 0u;
     sc = __byte_perm(pr, pr, 0x1010);
     ba = __byte_perm(pr, pr, 0x3232);
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Para
   const int64_t row0 = ((int64_t)s * P.width + page) * PAGE;
   {
     uint32_t sc, ba;
-    const bool past = past_range(params(0, kr, sc, ba));
+    const bool past = past_range(params(false, kr, sc, ba));
     uint4* dst = reinterpret_cast<uint4*>(k + ((row0 + kr) * P.a.hkv + h) * D + (ts & 3) * 32);
     const uint32_t* w = &kc.x;
 #pragma unroll
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(256) q4_expand_kv(const __grid_constant__ Para
   }
   {
     uint32_t s0, b0, s1, b1;
-    const uint32_t p0 = params(64, vr, s0, b0), p1 = params(64, vr + 1, s1, b1);
+    const uint32_t p0 = params(true, vr, s0, b0), p1 = params(true, vr + 1, s1, b1);
     const uint32_t sc = __byte_perm(s0, s1, 0x5410), ba = __byte_perm(b0, b1, 0x5410);
     const bool past = past_range(half2_max(p0, p1));
     uint4* d0 = reinterpret_cast<uint4*>(v + ((row0 + vr) * P.a.hkv + h) * D + ((ts & 31) >> 2) * 16);

@@ -142,3 +142,30 @@ def test_rows_that_reach_the_largest_fp16(kind, shape):
     k, v = c.rows(1)
     assert (k > 65520).any() and (v > 65520).any()
     c.check()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+@pytest.mark.parametrize("which", ["key", "value", "both"])
+def test_a_nan_row_spoils_only_rows_that_see_it(kind, shape, which):
+    """Late in a run's own rows, where the rows of one tile differ in what they see; and behind
+    the window of some of them."""
+    for mods in (dict(), dict(window=40), dict(softcap=5.0, prefix=[3, 0, 70])):
+        c = Case(81, **shape, **mods)
+        assert c.form() == kind
+        hit = [(s, n - 37) for s, n in enumerate(c.kv)]
+        clean = c.pool.copy()
+        for s, at in hit:
+            for par in {"key": [0], "value": [64], "both": [0, 64]}[which]:
+                first = 16 * D + par + 4 * (at % 16)
+                c.pool[c.tables[s, at // 16], 1, first:first + 4] = 0xFF
+        got = c.run().double().cpu().numpy()
+        K.check_device_errors()
+        c.pool = clean
+        want, tol, _ = c.want()
+        sees = np.concatenate([R.visible(c.ql, n, True, c.window, 0 if c.prefix is None else c.prefix[s])
+                               [:, at] for (s, at), n in zip(hit, c.kv)])
+        assert sees.any() and not sees.all()
+        group = np.arange(c.hq) // (c.hq // c.hkv) == 1   # the head whose row is NaN
+        assert np.isnan(got[sees][:, group]).all()
+        fine = ~(sees[:, None] & group)
+        assert np.isfinite(got[fine]).all() and (np.abs(got - want) <= tol)[fine].all()
