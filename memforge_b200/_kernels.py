@@ -682,16 +682,14 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
     if mods is not None:
         a.mods = mods
     lib = L.lib()
-    ws, nbytes = workspace_tensor, 0
+    ws, nbytes, fresh = workspace_tensor, 0, False
     if ws is None:
         key = (dev.index, code, D, hq, hkv, num_seqs, most, width, cu_seqlens_q is None,
                mods is None, rows, (a.q | a.out | 2 * (qs[0] | qs[1] | os_[0] | os_[1])) & 15)
         nbytes = _q4_need.get(key)
-        if nbytes is None:
+        fresh = nbytes is None
+        if fresh:
             nbytes = lib.mf_q4_paged_attention_workspace_size(a, dev.index)
-            if len(_q4_need) > 4096:
-                _q4_need.clear()
-            _q4_need[key] = nbytes
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     else:
@@ -704,6 +702,10 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
             rc = lib.mf_q4_paged_attention(*args)
     if rc:
         L.check(rc, "mf_q4_paged_attention")
+    if fresh:   # (not of a refused call, whose size of 0 says nothing)
+        if len(_q4_need) > 4096:
+            _q4_need.clear()
+        _q4_need[key] = nbytes
     launch_counter["q4_paged_attention"] += 1
     if _checks:
         _after("q4_paged_attention", dev)

@@ -1,0 +1,29 @@
+"""Calls of 4-bit attention at the edges of what is allowed: after a refused call, without rows."""
+
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_q4 import Case
+
+pytestmark = pytest.mark.gpu
+
+K = pytest.importorskip("memforge_b200._kernels")
+
+
+def test_a_refused_call_leaves_later_ones_as_they_were():
+    """A refused call says nothing about the workspace that a valid one of its sizes needs."""
+    for seed, hq, bad in ((200, 12, dict(scale=0.0)), (201, 20, dict(scale=math.nan))):
+        c = Case(seed, "bf16", hq, 4, 128, [333, 41, 97], [1] * 3)  # (sizes of no other test)
+        with pytest.raises(RuntimeError, match="scale"):
+            c.run(**bad)
+        c.check()
+    c = Case(202, "bf16", 28, 4, 128, [333, 41, 98], [1] * 3)
+    tables = torch.from_numpy(c.tables).cuda()
+    kv = torch.tensor(c.kv_lens, dtype=torch.int32).cuda()
+    room = torch.zeros(c.pool.size + 8, dtype=torch.uint8, device="cuda")
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        K.q4_paged_attention(c.q_dev, torch.empty_like(c.q_dev), room[8:].view(c.pool.shape), tables,
+                             kv, scale=c.scale)
+    c.check()
