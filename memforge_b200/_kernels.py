@@ -673,6 +673,8 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
     if not kv_lens.is_contiguous():
         kv_lens = kv_lens.contiguous()
     width, code = block_tables.shape[1], dtype_code(q.dtype)
+    if rows == 0:
+        return out
     a = L.Q4AttentionArgs(
         ctypes.sizeof(L.Q4AttentionArgs), q.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0],
         os_[1], ptr, sb, sh, nb, block_tables.data_ptr(), ts[0], width, _ptr(cu_seqlens_q),

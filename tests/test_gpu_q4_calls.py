@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from memforge_b200.quant_cache import paged_attention_q4
 from tests.test_gpu_q4 import Case
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,16 @@ def test_a_refused_call_leaves_later_ones_as_they_were():
         K.q4_paged_attention(c.q_dev, torch.empty_like(c.q_dev), room[8:].view(c.pool.shape), tables,
                              kv, scale=c.scale)
     c.check()
+
+
+def test_a_batch_without_rows_is_nothing_to_do():
+    pool = torch.zeros((2, 4, 2, 2176), dtype=torch.uint8, device="cuda")
+    q = torch.empty((0, 8, 128), dtype=torch.bfloat16, device="cuda")
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    tables = torch.zeros((3, 2), dtype=torch.int32, device="cuda")
+    kv, cu = tables[:, 0].contiguous(), torch.zeros(4, dtype=torch.int32, device="cuda")
+    assert paged_attention_q4(q, pool, 1, tables[:0], none).shape == (0, 8, 128)
+    assert paged_attention_q4(q, pool, 1, tables, kv, cu_seqlens_q=cu, max_q_len=0).shape == (0, 8, 128)
+    assert paged_attention_q4(q, pool, 1, tables, kv, cu_seqlens_q=cu, max_q_len=5).shape == (0, 8, 128)
+    with pytest.raises(ValueError, match="num_seqs"):
+        paged_attention_q4(q, pool, 1, tables[:2], kv, cu_seqlens_q=cu, max_q_len=0)
