@@ -1062,7 +1062,7 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
     return fail(MF_EINVAL, "q4 attention: pool base and strides must be multiples of 16 bytes");
   if (a->num_seqs > 65535) return fail(MF_EUNSUPPORTED, "q4 attention: more than 65535 sequences");
   if (a->num_seqs > 0 && a->total_q > 0 &&
-      (!a->q || !a->out || !a->pool || !a->block_tables || !a->kv_lens))
+      (!a->q || !a->out || !a->pool || (!a->block_tables && a->table_width > 0) || !a->kv_lens))
     return fail(MF_EINVAL, "q4 attention: null pointer");
   if (!softcap_ok(a->mods.softcap) || a->mods.window < 0)
     return fail(MF_EINVAL, "q4 attention: softcap must be 0 or from 1e-30 to 1e30, window not "

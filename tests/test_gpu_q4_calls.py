@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from memforge_b200.quant_cache import paged_attention_q4
+from tests.gpu_util import TORCH_DT
 from tests.test_gpu_q4 import Case
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,19 @@ def test_a_batch_without_rows_is_nothing_to_do():
     assert paged_attention_q4(q, pool, 1, tables, kv, cu_seqlens_q=cu, max_q_len=5).shape == (0, 8, 128)
     with pytest.raises(ValueError, match="num_seqs"):
         paged_attention_q4(q, pool, 1, tables[:2], kv, cu_seqlens_q=cu, max_q_len=0)
+
+
+@pytest.mark.parametrize("dtype,ql", [("bf16", 1), ("bf16", 300), ("f32", 3)])
+def test_tables_without_entries_are_contexts_without_keys(dtype, ql):
+    """No block for any sequence: every row is zeros; a length that would need one is reported."""
+    q = torch.ones((2 * ql, 16, 128), dtype=TORCH_DT[dtype], device="cuda")
+    pool = torch.zeros((4, 4, 2176), dtype=torch.uint8, device="cuda")
+    tables = torch.zeros((2, 0), dtype=torch.int32, device="cuda")
+    kv = torch.zeros(2, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    K.q4_paged_attention(q, out, pool, tables, kv, q_per_seq=ql, scale=0.1)
+    K.check_device_errors()
+    assert not out.any()
+    K.q4_paged_attention(q, out, pool, tables, kv + 1, q_per_seq=ql, scale=0.1)
+    with pytest.raises(IndexError, match="block table"):
+        K.check_device_errors()
