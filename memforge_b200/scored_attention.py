@@ -55,6 +55,8 @@ def paged_attention_scored(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
         q = q.contiguous()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if q.shape[0] == 0:
+        return out
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return K.paged_attention(q, out, key_pool[layer_idx], value_pool[layer_idx], block_tables,
