@@ -44,6 +44,7 @@ from typing import Any, List, Optional, Sequence, Tuple
 import torch
 
 from . import _kernels as K
+from .kv_pool import pool_attend, pool_kv_heads
 from .varlen_attention import _plan as _varlen_plan
 from .varlen_attention import _tables as _varlen_tables
 
@@ -138,7 +139,7 @@ class _VarlenBinding:
         if self._meta is None:
             plan, cu, kv, row_map, index = _varlen_plan(
                 len(self.seq_ids), self.block_tables, self.seq_ids, self.positions,
-                self.pool.block_size, num_heads, self.pool.spec.num_kv_heads, device)
+                self.pool.block_size, num_heads, pool_kv_heads(self.pool), device)
             tables = _varlen_tables(plan, self.block_tables, index, device)
             self._meta = _DeviceRows(tables, cu, kv, row_map, plan.max_q_len, plan.total,
                                      q_per_seq=plan.uniform_q)
@@ -215,11 +216,12 @@ def any_binding_active() -> bool:
 
 def _run(query_rows, out_rows, pool, layer_idx, meta: _DeviceRows, scale, mods):
     if meta.q_per_seq:
-        pool.attend(layer_idx, query_rows, out_rows, meta.tables, meta.kv,
+        pool_attend(pool, layer_idx, query_rows, out_rows, meta.tables, meta.kv,
                     q_per_seq=meta.q_per_seq, scale=scale, **mods)
     else:
-        pool.attend(layer_idx, query_rows, out_rows, meta.tables, meta.kv, cu_seqlens_q=meta.cu,
-                    max_q_len=meta.max_q, scale=scale, row_map=meta.row_map, **mods)
+        pool_attend(pool, layer_idx, query_rows, out_rows, meta.tables, meta.kv,
+                    cu_seqlens_q=meta.cu, max_q_len=meta.max_q, scale=scale, row_map=meta.row_map,
+                    **mods)
 
 
 def _score_mods(kwargs) -> dict:
@@ -259,8 +261,8 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
         if q_len != 1:
             raise ValueError(f"a graphed decode step has one query row per sequence, got "
                              f"{q_len}")
-        graph.pool.attend(module.layer_idx, query[:, :, 0], out[:, 0], graph.tables, graph.ctx,
-                          q_per_seq=1, scale=scale, causal=True, **mods)
+        pool_attend(graph.pool, module.layer_idx, query[:, :, 0], out[:, 0], graph.tables,
+                    graph.ctx, q_per_seq=1, scale=scale, causal=True, **mods)
         graph.used += 1
         return out, None
 

@@ -30,6 +30,7 @@ import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 from . import attention_backend as AB
+from .kv_pool import pool_device, pool_write_rows
 
 
 class _GraphLayer(CacheLayerMixin):
@@ -47,7 +48,7 @@ class _GraphLayer(CacheLayerMixin):
         o, l = self.owner, self.layer_idx
         b = o._b
         # (B, H, 1, D) -> (B, H, D) rows at each row's slot, this layer's pool
-        o.pool.write_rows(l, key_states[:, :, 0], value_states[:, :, 0], o._slots[:b])
+        pool_write_rows(o.pool, l, key_states[:, :, 0], value_states[:, :, 0], o._slots[:b])
         return key_states, value_states
 
     def get_seq_length(self) -> int:
@@ -76,7 +77,7 @@ class GraphedPagedDecoder:
         if not AB.register():
             raise RuntimeError("graphed paged decode needs the transformers attention registry")
         self.model, self.pool = model, pool
-        self.device = torch.device(pool.device)
+        self.device = torch.device(pool_device(pool))
         if self.device.type != "cuda":
             raise ValueError("graphed paged decode needs a CUDA device")
         self.bs = pool.block_size

@@ -18,6 +18,45 @@ from . import _kernels as K
 from . import paged_gather
 
 
+# What the cache, the attention function and the graphed decoder ask of a pool.  A pool that
+# holds rows in a form of its own brings attend, write_rows, device and spec (PagedKVPool,
+# Q4KVPool); of any other object, MemForge's own pool among them, key_pool, value_pool and
+# block_size are enough.
+
+def pool_device(pool) -> torch.device:
+    return pool.key_pool.device if hasattr(pool, "key_pool") else pool.device
+
+
+def pool_kv_heads(pool) -> int:
+    return pool.key_pool.shape[3] if hasattr(pool, "key_pool") else pool.spec.num_kv_heads
+
+
+def _write_rows(pool, layer_idx, keys, values, slots) -> None:
+    K.reshape_and_cache(keys, values, pool.key_pool[layer_idx], pool.value_pool[layer_idx], slots)
+
+
+def _attend(pool, layer_idx, q, out, block_tables, kv_lens, **how) -> torch.Tensor:
+    return K.paged_attention(q, out, pool.key_pool[layer_idx], pool.value_pool[layer_idx],
+                             block_tables, kv_lens, **how)
+
+
+def pool_write_rows(pool, layer_idx: int, keys: torch.Tensor, values: torch.Tensor,
+                    slots: torch.Tensor) -> None:
+    write = getattr(pool, "write_rows", None)
+    if write is None:
+        _write_rows(pool, layer_idx, keys, values, slots)
+    else:
+        write(layer_idx, keys, values, slots)
+
+
+def pool_attend(pool, layer_idx: int, q: torch.Tensor, out: torch.Tensor,
+                block_tables: torch.Tensor, kv_lens: torch.Tensor, **how) -> torch.Tensor:
+    attend = getattr(pool, "attend", None)
+    if attend is None:
+        return _attend(pool, layer_idx, q, out, block_tables, kv_lens, **how)
+    return attend(layer_idx, q, out, block_tables, kv_lens, **how)
+
+
 @dataclass(frozen=True)
 class ModelKVSpec:
     """Per-token KV geometry (``kv_pool.py:27-55``)."""
@@ -116,19 +155,17 @@ class PagedKVPool:
 
     @property
     def device(self) -> torch.device:
-        return self.key_pool.device
+        return pool_device(self)
 
     def write_rows(self, layer_idx: int, keys: torch.Tensor, values: torch.Tensor,
                    slots: torch.Tensor) -> None:
         """Scatter ``(T, H, D)`` rows at ``slots`` (device tensor; graph safe)."""
-        K.reshape_and_cache(keys, values, self.key_pool[layer_idx], self.value_pool[layer_idx],
-                            slots)
+        _write_rows(self, layer_idx, keys, values, slots)
 
     def attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor,
                block_tables: torch.Tensor, kv_lens: torch.Tensor, **how) -> torch.Tensor:
         """``_kernels.paged_attention`` of ``(rows, Hq, D)`` queries over one layer."""
-        return K.paged_attention(q, out, self.key_pool[layer_idx], self.value_pool[layer_idx],
-                                 block_tables, kv_lens, **how)
+        return _attend(self, layer_idx, q, out, block_tables, kv_lens, **how)
 
     def zero_(self) -> None:
         self.key_pool.zero_()

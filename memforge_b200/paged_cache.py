@@ -29,7 +29,7 @@ from typing import Dict, List, Optional, Tuple
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
-from .kv_pool import PagedKVPool
+from .kv_pool import PagedKVPool, pool_device
 
 
 class PagedCacheLayer(CacheLayerMixin):
@@ -271,7 +271,7 @@ class VarlenPackedCache(Cache):
         tables a slot named by two sequences is rejected too.
         """
         bs = self.pool.block_size
-        device = self.pool.device
+        device = pool_device(self.pool)
         sizes = [int(t.numel()) if hasattr(t, "numel") else len(t) for t in self.block_tables]
         offs = [0]
         for n in sizes:

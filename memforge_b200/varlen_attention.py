@@ -27,6 +27,7 @@ import numpy as np
 import torch
 
 from . import _kernels as K
+from .kv_pool import pool_attend, pool_kv_heads
 from .varlen_plan import VarlenPlan, group_by_sequence, plan_varlen  # noqa: F401
 
 MASK_FILL = float("-inf")
@@ -135,16 +136,14 @@ def paged_attention_varlen_materialised(query: torch.Tensor, pool, layer_idx: in
                                         scale: Optional[float] = None) -> torch.Tensor:
     """
     Same function as ``paged_attention_varlen`` (``varlen_attention.py:291-395``), over a
-    ``PagedKVPool`` or a 4-bit ``Q4KVPool``.
+    ``PagedKVPool``, an object with its ``key_pool``, ``value_pool`` and ``block_size``, or a
+    4-bit ``Q4KVPool``.
     On B200 nothing is materialised: both names run the same kernel.
     """
-    if not hasattr(pool, "attend"):
-        return paged_attention_varlen(query, pool.key_pool, pool.value_pool, layer_idx,
-                                      block_tables, seq_ids, positions, pool.block_size, scale)
     K.require_cuda("paged_attention_varlen", query)
 
     def attend(q, out, tables, kv, **how):
-        pool.attend(layer_idx, q, out, tables, kv, **how)
+        pool_attend(pool, layer_idx, q, out, tables, kv, **how)
 
-    return _run(query, attend, pool.spec.num_kv_heads, pool.block_size, block_tables, seq_ids,
+    return _run(query, attend, pool_kv_heads(pool), pool.block_size, block_tables, seq_ids,
                 positions, scale, pool.block_size)
