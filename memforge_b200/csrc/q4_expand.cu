@@ -31,19 +31,24 @@ __global__ void __launch_bounds__(THREADS, 1) q4_expanded_kernel(
 }
 
 // q in fp16, each row times the power of two that brings its largest element to
-// [2^14, 2^15), in the order of the run's rows; 16 lanes a row.
+// [2^14, 2^15), in the order of the run's rows; 16 lanes a row.  Rows of no sequence (behind the
+// last one's) become zeros: neither their entries of the row map nor their q are read.
 template <typename T>
 __global__ void __launch_bounds__(256) q4_expand_q(const __grid_constant__ Params P, __half* out,
                                                    float* scale) {
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t at = blockIdx.x * 16 + threadIdx.x / 16, rows = (uint32_t)(P.a.total_q * P.a.hq);
-  const bool have = at < rows;
   const int c = threadIdx.x & 15;
-  const uint32_t r = have ? at / (uint32_t)P.a.hq : 0, h = have ? at - r * (uint32_t)P.a.hq : 0;
-  const T* p = static_cast<const T*>(P.a.q) + (int64_t)map_row(P.a, (int)r) * P.a.q_sr +
-               (int64_t)h * P.a.q_sh + c * 8;
-  const uint4 in = __ldg(reinterpret_cast<const uint4*>(p));
+  const int r = (int)(at / (uint32_t)P.a.hq), h = (int)(at - (uint32_t)r * (uint32_t)P.a.hq);
+  const int first = P.a.cu_q ? P.a.cu_q[0] : 0;
+  const int end = P.a.cu_q ? P.a.cu_q[P.a.num_seqs] : P.a.num_seqs * P.a.q_per_seq;
+  uint4 in = make_uint4(0, 0, 0, 0);
+  if (at < rows && r >= first && r < end) {
+    const T* p = static_cast<const T*>(P.a.q) + (int64_t)map_row(P.a, r) * P.a.q_sr +
+                 (int64_t)h * P.a.q_sh + c * 8;
+    in = __ldg(reinterpret_cast<const uint4*>(p));
+  }
   const T* t = reinterpret_cast<const T*>(&in);
   float x[8];
 #pragma unroll
@@ -53,7 +58,7 @@ __global__ void __launch_bounds__(256) q4_expand_q(const __grid_constant__ Param
   for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (!have) return;
+  if (at >= rows) return;
   const int ex = (int)(__float_as_uint(top) >> 23);
   const float mul = __uint_as_float((uint32_t)min(max(268 - ex, 1), 240) << 23);
   if (c == 0) scale[at] = P.scale_log2 / mul;

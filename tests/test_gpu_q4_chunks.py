@@ -169,3 +169,26 @@ def test_a_nan_row_spoils_only_rows_that_see_it(kind, shape, which):
         assert np.isnan(got[sees][:, group]).all()
         fine = ~(sees[:, None] & group)
         assert np.isfinite(got[fine]).all() and (np.abs(got - want) <= tol)[fine].all()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+@pytest.mark.parametrize("pad", [-1, 10 ** 6])
+def test_entries_of_row_map_behind_the_last_sequence_are_not_followed(kind, shape, pad):
+    """A padded batch: rows behind the last sequence, whose entries name no row of q."""
+    c = Case(83, **shape)
+    rows, spare = len(c.kv) * c.ql, 37
+    perm = torch.from_numpy(rng(83).permutation(rows).astype(np.int32)).cuda()
+    q = torch.full((rows + spare, c.hq, D), math.nan, dtype=torch.bfloat16, device="cuda")
+    q[perm.long()] = c.q_dev
+    out = torch.full_like(q, 5.0)
+    row_map = torch.cat([perm, torch.full((spare,), pad, dtype=torch.int32, device="cuda")])
+    cu = torch.arange(len(c.kv) + 1, dtype=torch.int32, device="cuda") * c.ql
+    for how in (dict(), dict(cu_seqlens_q=cu, max_q_len=c.ql)):
+        if how:
+            c.run(q=q, out=out, row_map=row_map, **how)
+        else:   # (without offsets every row belongs to a sequence)
+            c.run(q=q[:rows], out=out[:rows], row_map=perm)
+        K.check_device_errors()
+        c.hold(out[perm.long()].double().cpu().numpy())
+        assert (out[rows:] == 5.0).all()
+        out.fill_(5.0)
