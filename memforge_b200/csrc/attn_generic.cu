@@ -96,21 +96,22 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
     // -2 - row for a window row, -1 for nothing (past the range / bad id).
     if (tid < GEN_TILE) {
       const int kpos = t0 + tid;
+      const int lb = kpos / p.block_size;
+      // A block that no row of the tile sees may have been freed: its entry is not read.
+      const bool hidden = MOD && lb * p.block_size >= pfx &&
+                          (int64_t)lb * p.block_size + p.block_size <= key_lo;
       int64_t off = -1;
-      if (kpos < key_end) {
+      if (kpos < key_end && !hidden) {
         if (wk && kpos >= win_start) {
           off = -2 - (int64_t)map_row(p, q_start + (kpos - win_start));
+        } else if (lb >= p.table_stride) {
+          set_err(p.err, MF_ERR_TABLE);
         } else {
-          const int lb = kpos / p.block_size;
-          if (lb >= p.table_stride) {
-            set_err(p.err, MF_ERR_TABLE);
+          const int blk = p.tables[(int64_t)s * p.table_stride + lb];
+          if (blk < 0 || blk >= p.num_blocks) {
+            set_err(p.err, MF_ERR_BLOCK_ID);
           } else {
-            const int blk = p.tables[(int64_t)s * p.table_stride + lb];
-            if (blk < 0 || blk >= p.num_blocks) {
-              set_err(p.err, MF_ERR_BLOCK_ID);
-            } else {
-              off = (int64_t)blk * p.sb + (int64_t)(kpos % p.block_size) * p.ss + (int64_t)h * p.sh;
-            }
+            off = (int64_t)blk * p.sb + (int64_t)(kpos % p.block_size) * p.ss + (int64_t)h * p.sh;
           }
         }
       }

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from memforge_b200.scored_attention import paged_attention_scored
+from tests.test_gpu_scored import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -16,3 +17,23 @@ def test_a_batch_without_rows_is_nothing_to_do():
     for how in (dict(window=5), dict(softcap=3.0), dict()):
         out = paged_attention_scored(q, pool, pool, 1, tables, kv, cu_seqlens_q=cu, max_q_len=4, **how)
         assert out.shape == (0, 8, 128)
+
+
+@pytest.mark.parametrize("dtype,hq,d,ql,block", [("f32", 4, 80, 1, 16), ("f32", 4, 128, 3, 8),
+                                                 ("bf16", 4, 256, 40, 16), ("f32", 4, 64, 20, 4),
+                                                 ("bf16", 4, 128, 1, 16), ("bf16", 4, 128, 90, 16)])
+@pytest.mark.parametrize("prefix", [0, 5, 36])
+def test_blocks_behind_a_window_may_be_freed(dtype, hq, d, ql, block, prefix):
+    """Table entries of blocks that no row sees are not read: -1 there is no error."""
+    c = Case(240, dtype, hq, 2, d, [ql + 150, ql + 39, ql + 77], [ql] * 3, window=13, block=block,
+             prefix=[prefix] * 3 if prefix else None)
+    freed = 0
+    for s, n in enumerate(c.kv_lens):
+        low = n - ql - 13 + 1
+        for b in range(low // block):
+            if b * block >= prefix:
+                c.tables[s, b] = -1
+                freed += 1
+    assert freed > 3
+    # (the reference below reads block -1, the last one: its rows are hidden)
+    c.check()
