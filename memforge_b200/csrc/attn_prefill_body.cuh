@@ -287,18 +287,19 @@ constexpr float CAP2[5] = {0.9999972283095431f, -0.33323076454511924f, 0.1322609
 
 // sv = capped scores in log2 units, of raw scores (times sl2: log2 units).  The polynomial's
 // factors take in sl2 and the cap, so the short one is four packed operations a pair; the
-// largest score of the warp's rows decides.
+// largest score of the warp's rows decides, and that its factors are finite: under a cap far
+// below any score (1e-12, say) they are not, and a score of 0 would come out as NaN.
 template <int N>
 MF_DEVINL void cap_scores(const Params& P, float* sv, float sl2) {
-  const float ky = sl2 * P.inv_cap2;
+  const float ky = fminf(sl2 * P.inv_cap2, 1e30f);
   float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < N; c += 2)
     top[(c >> 1) & 3] = fmax3f(top[(c >> 1) & 3], fabsf(sv[c]), fabsf(sv[c + 1]));
   const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * ky;
-  if (!__any_sync(0xffffffffu, mx > CAP_MAX1)) {
-    const float k2 = ky * ky;
-    const float f0 = CAP1[0] * sl2, f1 = CAP1[1] * sl2 * k2, f2 = CAP1[2] * sl2 * k2 * k2;
+  const float k2 = ky * ky;
+  const float f0 = CAP1[0] * sl2, f1 = CAP1[1] * sl2 * k2, f2 = CAP1[2] * sl2 * k2 * k2;
+  if (!__any_sync(0xffffffffu, mx > CAP_MAX1 || f2 > 1e38f)) {
     const uint64_t c0 = f32x2(f0, f0), c1 = f32x2(f1, f1), c2 = f32x2(f2, f2);
 #pragma unroll
     for (int c = 0; c < N; c += 2) {

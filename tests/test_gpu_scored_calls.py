@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from memforge_b200.scored_attention import paged_attention_scored
+from tests.test_gpu_q4 import Case as Q4Case
 from tests.test_gpu_scored import Case
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +38,14 @@ def test_blocks_behind_a_window_may_be_freed(dtype, hq, d, ql, block, prefix):
     assert freed > 3
     # (the reference below reads block -1, the last one: its rows are hidden)
     c.check()
+
+
+@pytest.mark.parametrize("softcap", [1e-30, 1e-20, 1e-12, 1e-6, 50.0, 1e30])
+@pytest.mark.parametrize("dtype,hq,d,ql", [("bf16", 16, 128, 200), ("f16", 8, 128, 1),
+                                           ("bf16", 8, 128, 20), ("f32", 4, 80, 3)])
+def test_scores_of_zero_under_any_cap(softcap, dtype, hq, d, ql):
+    """A zero query weighs its keys alike, however small the cap is."""
+    c = Case(241, dtype, hq, 4, d, [ql + 60, ql + 200], [ql] * 2, softcap=softcap, q_scale=0.0)
+    c.check()
+    if d == 128:
+        Q4Case(242, dtype, hq, 4, d, [ql + 60, ql + 200], [ql] * 2, softcap=softcap, q_scale=0.0).check()
