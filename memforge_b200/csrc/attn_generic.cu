@@ -164,8 +164,12 @@ __global__ void __launch_bounds__(GEN_WARPS * 32)
       float tmax = sc;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
-      const float m_new = fmaxf(m[k], tmax);
-      if (m_new == -INFINITY) continue;  // nothing visible yet (cannot happen past tile 0)
+      float m_new = fmaxf(m[k], tmax);
+      if (m_new == -INFINITY) {  // nothing visible yet
+        // (MOD: or only scores of NaN, which a maximum passes over; they spoil the row)
+        if (!MOD || !__any_sync(0xffffffffu, sc != sc)) continue;
+        m_new = 0.f;
+      }
       const float alpha = (m[k] == -INFINITY) ? 0.f : expf(m[k] - m_new);
       const float pj = see ? expf(sc - m_new) : 0.f;
       float psum = pj;

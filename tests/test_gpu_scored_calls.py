@@ -1,5 +1,8 @@
 """Calls of attention with modified scores at the edges of what is allowed."""
 
+import math
+
+import numpy as np
 import pytest
 import torch
 
@@ -49,3 +52,16 @@ def test_scores_of_zero_under_any_cap(softcap, dtype, hq, d, ql):
     c.check()
     if d == 128:
         Q4Case(242, dtype, hq, 4, d, [ql + 60, ql + 200], [ql] * 2, softcap=softcap, q_scale=0.0).check()
+
+
+@pytest.mark.parametrize("dtype,hq,d,ql", [("bf16", 8, 128, 1), ("f16", 8, 64, 1), ("bf16", 8, 128, 5),
+                                           ("bf16", 16, 128, 40), ("f32", 4, 80, 3),
+                                           ("bf16", 4, 256, 2)])
+def test_a_row_that_sees_only_nan_keys_is_nan(dtype, hq, d, ql):
+    c = Case(243, dtype, hq, 4, d, [ql, ql + 40], [ql] * 2, window=1)
+    slots = c.tables[0, np.arange(ql) // 16] * 16 + np.arange(ql) % 16
+    c.k_dev.view(-1, 4, d)[torch.from_numpy(slots).cuda().long()] = math.nan
+    got = c.run().double().cpu().numpy()
+    want, tol = c.want()
+    assert np.isnan(got[:ql]).all()
+    assert (np.abs(got - want)[ql:] <= tol[ql:]).all()
