@@ -423,7 +423,18 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, key_pool: torch.Tensor,
     mods = score_mods(dev, hq, num_seqs, softcap, window, alibi_slopes, prefix_lens)
     if mods is not None:
         require_one_device("paged_attention", dev, out, key_pool, value_pool, block_tables,
-                           kv_lens, cu_seqlens_q, row_map)
+                           kv_lens, cu_seqlens_q, row_map, workspace_tensor)
+        if out.shape != q.shape or value_pool.shape != key_pool.shape:
+            raise ValueError(f"out must have q's shape and the value pool the key pool's, got "
+                             f"{tuple(out.shape)} for {tuple(q.shape)} and "
+                             f"{tuple(value_pool.shape)} for {tuple(key_pool.shape)}")
+        if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs:
+            raise ValueError("block_tables must be [num_seqs, width]")
+        if cu_seqlens_q is not None and (cu_seqlens_q.numel() != num_seqs + 1 or max_q_len is None
+                                         or not cu_seqlens_q.is_contiguous()):
+            raise ValueError("cu_seqlens_q needs num_seqs + 1 contiguous offsets and max_q_len")
+        if row_map is not None and (row_map.numel() < rows or not row_map.is_contiguous()):
+            raise ValueError("row_map must be contiguous with an entry for each row")
         with _on(dev):
             need = lib.mf_paged_attention_scored_workspace_size(a, mods, idx)
             ws = workspace_tensor if workspace_tensor is not None else (

@@ -12,6 +12,8 @@ from tests.test_gpu_scored import Case
 
 pytestmark = pytest.mark.gpu
 
+K = pytest.importorskip("memforge_b200._kernels")
+
 
 def test_a_batch_without_rows_is_nothing_to_do():
     pool = torch.zeros((2, 4, 16, 2, 128), dtype=torch.bfloat16, device="cuda")
@@ -65,3 +67,26 @@ def test_a_row_that_sees_only_nan_keys_is_nan(dtype, hq, d, ql):
     want, tol = c.want()
     assert np.isnan(got[:ql]).all()
     assert (np.abs(got - want)[ql:] <= tol[ql:]).all()
+
+
+def test_tensors_that_do_not_fit_the_call_are_refused():
+    """Before any launch: the kernels would read or write past them."""
+    c = Case(244, "bf16", 8, 2, 128, [50, 20, 33], [1] * 3, window=9)
+    tables = torch.from_numpy(c.tables).cuda()
+    kv = torch.tensor(c.kv_lens, dtype=torch.int32).cuda()
+    cu = torch.arange(4, dtype=torch.int32, device="cuda")
+
+    def call(out=None, v=None, t=None, **how):
+        out = torch.empty_like(c.q_dev) if out is None else out
+        return K.paged_attention(c.q_dev, out, c.k_dev, c.v_dev if v is None else v,
+                                 tables if t is None else t, kv, scale=c.scale, window=9, **how)
+
+    call(cu_seqlens_q=cu, max_q_len=1, row_map=cu[:3])
+    short = torch.empty_like(c.q_dev)
+    for bad in (dict(out=short[:2]), dict(out=short[:, :4]), dict(v=c.v_dev[:-1]), dict(t=tables[:2]),
+                dict(t=tables[0]), dict(cu_seqlens_q=cu[:3], max_q_len=1), dict(cu_seqlens_q=cu),
+                dict(cu_seqlens_q=torch.arange(8, dtype=torch.int32, device="cuda")[::2], max_q_len=1),
+                dict(row_map=cu[:2]), dict(row_map=torch.zeros(6, dtype=torch.int32, device="cuda")[::2])):
+        with pytest.raises(ValueError):
+            call(**bad)
+    K.check_device_errors()
