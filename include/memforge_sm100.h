@@ -459,6 +459,10 @@ MF_API int mf_q4_gather_kv(const void* pool, int64_t pool_stride_block, int64_t 
  *
  * The workspace (16-byte aligned) is scratch: it needs no initial value and nothing
  * in it outlives the call, but calls that may overlap must not share one.
+ *
+ * Long bf16 runs read a copy of the cache expanded to fp16, which makes up most of the
+ * workspace (up to 1 GiB).  With a smaller workspace, of the minimal size at least, they convert
+ * the records as they go: the same result up to rounding, in more time.
  */
 typedef struct {
   uint32_t struct_size; /* sizeof(mf_q4_attention_args) */
@@ -485,6 +489,8 @@ typedef struct {
 } mf_q4_attention_args;
 
 MF_API size_t mf_q4_paged_attention_workspace_size(const mf_q4_attention_args* args, int device);
+MF_API size_t mf_q4_paged_attention_min_workspace_size(const mf_q4_attention_args* args,
+                                                       int device);
 MF_API int mf_q4_paged_attention(const mf_q4_attention_args* args, void* workspace,
                                  size_t workspace_bytes, int32_t* err_flag, mf_stream_t stream);
 

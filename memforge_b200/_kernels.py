@@ -640,7 +640,8 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
     and head strides, D contiguous), one 4-bit pool layer (``layer``: of a pool with a
     layer dimension), and tables, lengths, rows and score modifiers as in
     :func:`paged_attention`.  The workspace is scratch of the caching allocator unless
-    one is given.
+    one is given; where it has no room for the expanded copy that long runs read, they
+    convert the cache as they go.
     """
     dev = q.device
     require_one_device("q4_paged_attention", dev, q, out, pool, block_tables, kv_lens,
@@ -704,7 +705,15 @@ def q4_paged_attention(q: torch.Tensor, out: torch.Tensor, pool: torch.Tensor,
         if fresh:
             nbytes = lib.mf_q4_paged_attention_workspace_size(a, dev.index)
         if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            try:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            except torch.OutOfMemoryError:
+                least = lib.mf_q4_paged_attention_min_workspace_size(a, dev.index)
+                if least >= nbytes:
+                    raise
+                # no room for the expanded copy (and it is not kept as the size of such calls)
+                nbytes, fresh = least, False
+                ws = torch.empty(least, dtype=torch.uint8, device=dev) if least else None
     else:
         nbytes = ws.numel() * ws.element_size()
     args = (a, _ptr(ws), nbytes, _err_ptr(dev), _stream_ptr(dev))

@@ -48,7 +48,8 @@ EXPORTED = (
     "mf_ipc_open", "mf_ipc_close", "mf_commit_window", "mf_gather_kv", "mf_accept_commit",
     "mf_paged_attention_scored_workspace_size", "mf_paged_attention_scored",
     "mf_q4_record_bytes", "mf_q4_reshape_and_cache", "mf_q4_gather_kv",
-    "mf_q4_paged_attention_workspace_size", "mf_q4_paged_attention",
+    "mf_q4_paged_attention_workspace_size", "mf_q4_paged_attention_min_workspace_size",
+    "mf_q4_paged_attention",
 )
 
 MF_IPC_HANDLE_BYTES = 64
@@ -183,11 +184,12 @@ def _declare(lib):
     lib.mf_q4_gather_kv.argtypes = [
         c_vp, c_i64, c_i64, c_i32, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, ctypes.c_int,
         c_i64, c_i64, c_vp, c_vp]
-    lib.mf_q4_paged_attention_workspace_size.argtypes = [ctypes.POINTER(Q4AttentionArgs),
-                                                         ctypes.c_int]
+    for size in (lib.mf_q4_paged_attention_workspace_size,
+                 lib.mf_q4_paged_attention_min_workspace_size):
+        size.argtypes = [ctypes.POINTER(Q4AttentionArgs), ctypes.c_int]
     lib.mf_q4_paged_attention.argtypes = [ctypes.POINTER(Q4AttentionArgs), c_vp, c_sz, c_vp, c_vp]
     sizes = ("mf_paged_attention_workspace_size", "mf_paged_attention_scored_workspace_size",
-             "mf_q4_paged_attention_workspace_size")
+             "mf_q4_paged_attention_workspace_size", "mf_q4_paged_attention_min_workspace_size")
     for name in sizes:
         getattr(lib, name).restype = c_sz
     lib.mf_q4_record_bytes.restype = c_i64

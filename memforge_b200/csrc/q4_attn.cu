@@ -1113,12 +1113,13 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
   return MF_OK;
 }
 
-Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
+// expand: may long runs read an expanded copy of the cache (else they convert as they go)
+Plan make_plan(q4a::Params& P, mf_dtype dt, int sms, bool expand = true) {
   Plan pl{};
   int64_t rows = (int64_t)P.a.max_q_len * P.G;
   pl.chunks = P.width > 0 && chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
   pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
-  pl.expand = pl.chunks && q4_expand_plan(P.a, P.width, P.vec, dt, pl.scratch);
+  pl.expand = expand && pl.chunks && q4_expand_plan(P.a, P.width, P.vec, dt, pl.scratch);
   if (!pl.tiles) {
     if (pl.expand) pl.ws_bytes = pl.scratch.bytes;
     return pl;
@@ -1155,14 +1156,23 @@ Plan make_plan(q4a::Params& P, mf_dtype dt, int sms) {
 
 using namespace mf;
 
-extern "C" size_t mf_q4_paged_attention_workspace_size(const mf_q4_attention_args* args,
-                                                       int device) {
+static size_t q4_workspace_bytes(const mf_q4_attention_args* args, int device, bool expand) {
   q4a::Params P;
   int sms = 0;
   if (to_q4_params(args, nullptr, P) != MF_OK || P.a.num_seqs == 0 || P.a.total_q == 0 ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
     return 0;
-  return make_plan(P, args->dtype, sms).ws_bytes;
+  return make_plan(P, args->dtype, sms, expand).ws_bytes;
+}
+
+extern "C" size_t mf_q4_paged_attention_workspace_size(const mf_q4_attention_args* args,
+                                                       int device) {
+  return q4_workspace_bytes(args, device, true);
+}
+
+extern "C" size_t mf_q4_paged_attention_min_workspace_size(const mf_q4_attention_args* args,
+                                                           int device) {
+  return q4_workspace_bytes(args, device, false);
 }
 
 extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* workspace,
@@ -1172,7 +1182,9 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
   const int rc = to_q4_params(args, err_flag, P);
   if (rc != MF_OK) return rc;
   if (P.a.num_seqs == 0 || P.a.total_q == 0 || P.a.max_q_len == 0) return MF_OK;
-  const Plan pl = make_plan(P, args->dtype, current_sm_count());
+  Plan pl = make_plan(P, args->dtype, current_sm_count());
+  if (pl.expand && workspace_bytes < pl.ws_bytes)
+    pl = make_plan(P, args->dtype, current_sm_count(), false);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (pl.tiles && (double)pl.rt * P.a.hkv * P.a.num_seqs * P.width >= 2147483648.0)
     return fail(MF_EUNSUPPORTED, "q4 attention: the tables could hold 2^31 or more (row tile, "
@@ -1180,7 +1192,7 @@ extern "C" int mf_q4_paged_attention(const mf_q4_attention_args* args, void* wor
   if (pl.ws_bytes > 0 && (!workspace || workspace_bytes < pl.ws_bytes ||
                           (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail(MF_EWORKSPACE, "q4 attention: workspace missing, misaligned or smaller than "
-                               "mf_q4_paged_attention_workspace_size()");
+                               "mf_q4_paged_attention_min_workspace_size()");
   P.prefix = static_cast<int32_t*>(workspace);
   if (pl.tiles) P.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.prefix_bytes);
   P.part_floats = pl.part_floats;

@@ -192,3 +192,29 @@ def test_entries_of_row_map_behind_the_last_sequence_are_not_followed(kind, shap
         c.hold(out[perm.long()].double().cpu().numpy())
         assert (out[rows:] == 5.0).all()
         out.fill_(5.0)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_without_room_for_the_expanded_copy_runs_convert(ragged, monkeypatch):
+    c = Case(84, **EXPANDED)
+    assert c.form() == "expanded"
+    how = dict(cu_seqlens_q=torch.arange(4, dtype=torch.int32, device="cuda") * c.ql,
+               max_q_len=c.ql) if ragged else dict()
+    real, refused = torch.empty, []
+
+    def empty(*size, **kw):
+        if kw.get("dtype") == torch.uint8 and size[0] > 4 << 20:
+            refused.append(size[0])
+            raise torch.OutOfMemoryError("no room")
+        return real(*size, **kw)
+
+    room = c.run(**how)
+    monkeypatch.setattr(torch, "empty", empty)
+    got = c.run(**how)
+    assert len(refused) == 1
+    monkeypatch.undo()
+    K.check_device_errors()
+    c.hold(got.double().cpu().numpy())
+    assert torch.equal(c.run(**how), room)   # with room again: as before
+    if not ragged:   # a given workspace that is too small for the copy
+        assert torch.equal(c.run(workspace_tensor=torch.empty(64, dtype=torch.uint8, device="cuda")), got)
