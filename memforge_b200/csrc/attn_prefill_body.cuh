@@ -75,7 +75,7 @@ constexpr int Q4_MMA_WARP = SM_WARPS, Q4_PV_WARP = SM_WARPS + 1, Q4_LOAD_WARP = 
 constexpr int Q4_CW = 4;  // converter warps of each kind
 constexpr int Q4_THREADS = (SM_WARPS + 4 + 2 * Q4_CW) * 32;
 // Registers: 640 threads start with 96 each; 256 * 168 + 384 * 48 is the same sum (the
-// launch checks that the kernel was built with 96).
+// plan checks that the kernel was built with 96).
 constexpr int Q4_REGS_LAUNCH = 96, Q4_REGS_SOFTMAX = 168, Q4_REGS_REST = 48;
 static_assert(Q4_THREADS * Q4_REGS_LAUNCH ==
                   SM_WARPS * 32 * Q4_REGS_SOFTMAX + (Q4_THREADS - SM_WARPS * 32) * Q4_REGS_REST,

@@ -1118,8 +1118,9 @@ Plan make_plan(q4a::Params& P, mf_dtype dt, int sms, bool expand = true) {
   Plan pl{};
   int64_t rows = (int64_t)P.a.max_q_len * P.G;
   pl.chunks = P.width > 0 && chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
-  pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
   pl.expand = expand && pl.chunks && q4_expand_plan(P.a, P.width, P.vec, dt, pl.scratch);
+  pl.chunks = pl.chunks && (pl.expand || q4_converting_built());
+  pl.tiles = !pl.chunks || P.a.cu_q;  // without offsets every run has max_q_len rows
   if (!pl.tiles) {
     if (pl.expand) pl.ws_bytes = pl.scratch.bytes;
     return pl;

@@ -8,6 +8,9 @@ namespace mf {
 // Whether the tcgen05 kernel takes runs of this call (the rest stay with mma.sync).
 bool q4_prefill_serves(const AttnParams& a, mf_dtype dtype);
 
+// Whether the converting form may run in this build.
+bool q4_converting_built();
+
 // Serves every sequence with more than rows_cap rows per kv head.  a.kp: the pool, a.sb /
 // a.sh its strides in bytes; width: entries of a block table's row; vec: q and out rows
 // allow 16-byte accesses.

@@ -2,6 +2,7 @@
 // convert from the records (attn_prefill_body.cuh, Q4).
 
 #include <algorithm>
+#include <atomic>
 
 #include "attn_prefill_body.cuh"
 #include "q4_attn.h"
@@ -22,14 +23,8 @@ static int launch_q4(const Params& P, int64_t grid, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (ready != dev) {
-    cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, kern);
-    if (e == cudaSuccess && at.numRegs != Q4_REGS_LAUNCH)
-      return fail(MF_EUNSUPPORTED, "q4 attention: the chunk kernel's register split does not "
-                                   "match its build");
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(smem_bytes(Q4_MAX_SEQS, true) + 1024));
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(smem_bytes(Q4_MAX_SEQS, true) + 1024));
     if (e != cudaSuccess)
       return fail(MF_ECUDA, std::string("q4 attention: ") + cudaGetErrorString(e));
     ready = dev;
@@ -58,6 +53,25 @@ static int launch_q4(const Params& P, int64_t grid, cudaStream_t stream) {
 bool q4_prefill_serves(const AttnParams& a, mf_dtype dtype) {
   return dtype == MF_BF16 && a.d == pf::D && a.hq / a.hkv <= pf::BM &&
          a.num_seqs <= pf::Q4_MAX_SEQS;
+}
+
+// The kernel's register split is of the 96 registers a thread that ptxas gave it here; a build
+// with another number must not run it (setmaxnreg would wait for registers that are not there), and
+// leaves such runs to mma.sync.
+bool q4_converting_built() {
+  static std::atomic<int> known{-1};
+  int ok = known.load(std::memory_order_relaxed);
+  if (ok < 0) {
+    cudaFuncAttributes a, b;
+    if (cudaFuncGetAttributes(&a, pf::q4_prefill_kernel<__nv_bfloat16, false>) != cudaSuccess ||
+        cudaFuncGetAttributes(&b, pf::q4_prefill_kernel<__nv_bfloat16, true>) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    ok = a.numRegs == pf::Q4_REGS_LAUNCH && b.numRegs == pf::Q4_REGS_LAUNCH;
+    known.store(ok, std::memory_order_relaxed);
+  }
+  return ok != 0;
 }
 
 int launch_q4_prefill(const AttnParams& a, int width, int vec, int rows_cap,

@@ -24,8 +24,8 @@ D = 128
 
 
 def form(num_seqs, q_per_seq, hq, hkv, width, rows):
-    """Which kernel a call of equal runs takes: the workspace tells.  Converting needs none, the
-    expanded copy takes 512 bytes a token and kv head, the mma.sync kernel its partial results."""
+    """Which kernel a call of equal runs takes: the workspace tells.  The mma.sync kernel needs
+    some, converting none, and an expanded copy is what it may do without."""
     a = L.Q4AttentionArgs()
     a.struct_size = ctypes.sizeof(a)
     a.q = a.out = a.pool = a.block_tables = a.kv_lens = 0x1000
@@ -36,9 +36,9 @@ def form(num_seqs, q_per_seq, hq, hkv, width, rows):
     a.q_per_seq, a.num_seqs, a.total_q, a.max_q_len = q_per_seq, num_seqs, rows, q_per_seq
     a.num_q_heads, a.num_kv_heads, a.head_dim = hq, hkv, D
     a.scale, a.causal, a.dtype = 0.1, 1, L.MF_BF16
-    need = L.lib().mf_q4_paged_attention_workspace_size(a, 0)
-    copy = 512 * num_seqs * width * 16 * hkv
-    return "converting" if need == 0 else "expanded" if need >= copy else "mma.sync"
+    need, least = (f(a, 0) for f in (L.lib().mf_q4_paged_attention_workspace_size,
+                                     L.lib().mf_q4_paged_attention_min_workspace_size))
+    return "expanded" if need > least else "converting" if need == 0 else "mma.sync"
 
 
 CONVERTING = dict(hq=16, hkv=4, kv=[200, 527, 640], ql=150)   # 60 row tiles of 16 a head, 5 of 128
