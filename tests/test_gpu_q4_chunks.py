@@ -218,3 +218,162 @@ def test_without_room_for_the_expanded_copy_runs_convert(ragged, monkeypatch):
     assert torch.equal(c.run(**how), room)   # with room again: as before
     if not ragged:   # a given workspace that is too small for the copy
         assert torch.equal(c.run(workspace_tensor=torch.empty(64, dtype=torch.uint8, device="cuda")), got)
+
+
+MODS = [dict(softcap=4.0), dict(slopes=True), dict(window=130, prefix=[20, 300, 0]), dict(window=1),
+        dict(softcap=2.0, window=33, slopes=True, prefix=[3, 64, 16])]
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+@pytest.mark.parametrize("mods", MODS)
+def test_modified_scores(kind, shape, mods):
+    c = Case(85, **shape, **mods)
+    assert c.form() == kind
+    c.check()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+@pytest.mark.parametrize("window", [1, 16, 17, 127, 128, 129, 300])
+def test_windows_and_prefixes_around_pages_and_tiles(kind, shape, window):
+    Case(86, **shape, window=window).check()
+    Case(87, **shape, window=window, prefix=[128, 1, 600]).check()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_non_causal_and_contexts_shorter_than_their_rows(kind, shape):
+    shape = dict(shape, kv=[0, 130, 400])
+    c = Case(88, **shape)
+    assert c.form() == kind
+    got = c.check()
+    ql = shape["ql"]
+    assert not got[:ql].any() and not got[ql:2 * ql - 130].any() and got[2 * ql - 130].any()
+    Case(89, **shape, causal=False).check()
+
+
+@pytest.mark.parametrize("kind,hq,hkv,ql", [
+    ("converting", 4, 4, 700), ("converting", 28, 4, 100), ("converting", 40, 5, 80),
+    ("converting", 96, 3, 60), ("converting", 128, 4, 23), ("converting", 84, 4, 40),
+    ("expanded", 4, 4, 800), ("expanded", 28, 4, 120), ("expanded", 80, 5, 56),
+    ("expanded", 27, 3, 300)])
+def test_every_group_size(kind, hq, hkv, ql):
+    c = Case(90, hq, hkv, [ql + 5, ql + 300, ql], ql)
+    assert c.form() == kind
+    c.check()
+
+
+@pytest.mark.parametrize("shape", [CONVERTING, EXPANDED])
+@pytest.mark.parametrize("mods", [dict(), dict(softcap=3.0, window=70)])
+def test_rows_without_alignment(shape, mods):
+    """Odd strides of q and out, rows in another order and rows of no sequence: element by
+    element, which only the converting form does."""
+    c = Case(91, **shape, **mods)
+    rows = len(c.kv) * c.ql
+    perm = torch.from_numpy(rng(91).permutation(rows).astype(np.int32)).cuda()
+    q = torch.full((rows + 9, c.hq, 131), math.nan, dtype=torch.bfloat16, device="cuda")
+    q[perm.long(), :, 1:129] = c.q_dev
+    out = torch.full((rows + 9, c.hq, 133), 5.0, dtype=torch.bfloat16, device="cuda")
+    row_map = torch.cat([perm, torch.full((9,), -1, dtype=torch.int32, device="cuda")])
+    cu = torch.arange(len(c.kv) + 1, dtype=torch.int32, device="cuda") * c.ql
+    c.run(q=q[:, :, 1:129], out=out[:, :, 2:130], row_map=row_map, cu_seqlens_q=cu, max_q_len=c.ql)
+    K.check_device_errors()
+    c.hold(out[perm.long(), :, 2:130].double().cpu().numpy())
+    assert (out[rows:] == 5.0).all() and (out[:, :, :2] == 5.0).all() and (out[:, :, 130:] == 5.0).all()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_ragged_runs_beside_short_and_empty_ones(kind, shape):
+    """One call's long runs take the chunk kernel, its short ones mma.sync."""
+    c = Case(92, **shape)
+    lens = [c.ql, 3, 0, c.ql - 50]
+    kv = [c.kv[2], 90, 40, c.kv[1]]
+    part = Case(92, c.hq, c.hkv, kv, c.ql)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32).cuda()
+    rows = sum(lens)
+    out = torch.full((rows + 2, c.hq, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    q = part.q_dev[:rows + 2]
+    part.run(q=q, out=out, cu_seqlens_q=cu, max_q_len=c.ql)
+    K.check_device_errors()
+    got, at = out.double().cpu().numpy(), 0
+    for s, n in enumerate(lens):
+        k, v = part.rows(s)
+        see = R.visible(n, kv[s])
+        o, mag, size = B.attention(part.q[at:at + n], B.operand(k), B.operand(v), part.scale, see)
+        if n > 8:
+            tol = B.chunk_bound("bf16", o, mag, size, kv[s], D, v_top=np.abs(v).max())
+            assert (np.abs(got[at:at + n] - o) <= tol).all()
+        elif n:
+            assert B.rms(got[at:at + n] - o) <= B.RMS["bf16"] * B.rms(o)
+        at += n
+    assert (out[rows:] == 5.0).all()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_graphs_on_two_streams_and_new_lengths(kind, shape):
+    c = Case(93, **shape)
+    pool, tables, kv = c.device()
+    how, graphs, outs = c.args(), [], []
+    K.q4_paged_attention(c.q_dev, torch.empty_like(c.q_dev), pool, tables, kv, **how)
+    for _ in range(2):
+        g, out = torch.cuda.CUDAGraph(), torch.empty_like(c.q_dev)
+        with torch.cuda.graph(g):
+            K.q4_paged_attention(c.q_dev, out, pool, tables, kv, **how)
+        graphs.append(g)
+        outs.append(out)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    c.hold(outs[0].double().cpu().numpy())
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], c.run())
+    kv.copy_(torch.tensor([160, 512, 0], dtype=torch.int32))   # (the poison lies behind these)
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    c.kv = [160, 512, 0]
+    c.hold(outs[1].double().cpu().numpy())
+    K.check_device_errors()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_reports(kind, shape):
+    """A block id outside the pool, a table too short for the length, a run longer than declared,
+    a negative length: reported, and the other sequences' rows as they are."""
+    c = Case(94, **shape)
+    want = c.run()
+    ql, keep = c.ql, c.tables.copy()
+
+    def others(out):
+        return torch.equal(out[:ql], want[:ql]) and torch.equal(out[2 * ql:], want[2 * ql:])
+
+    for bad in (-5, c.pool.shape[0]):
+        c.tables[1, 3] = bad
+        out = c.run()
+        with pytest.raises(IndexError, match="block table entry"):
+            K.check_device_errors()
+        assert others(out)
+    c.tables = keep
+    out = torch.full_like(c.q_dev, 5.0)
+    K.q4_paged_attention(c.q_dev, out, c.device()[0], torch.from_numpy(keep[:, :34]).cuda(),
+                         torch.tensor(c.kv, dtype=torch.int32).cuda(), **c.args())
+    with pytest.raises(IndexError, match="block table"):
+        K.check_device_errors()
+    assert torch.equal(out[:2 * ql], want[:2 * ql])   # (640 tokens need 40 entries)
+    cu = torch.tensor([0, ql, 2 * ql + 20, 3 * ql], dtype=torch.int32, device="cuda")
+    out = c.run(cu_seqlens_q=cu, max_q_len=ql, out=torch.full_like(c.q_dev, 5.0))
+    with pytest.raises(IndexError, match="length"):
+        K.check_device_errors()
+    assert torch.equal(out[:ql], want[:ql]) and (out[2 * ql:2 * ql + 20] == 5.0).all()
+    c.kv[1] = -3
+    out = c.run()
+    with pytest.raises(IndexError, match="length"):
+        K.check_device_errors()
+    assert others(out) and not out[ql:2 * ql].any()
+
+
+@pytest.mark.parametrize("kind,shape", FORMS)
+def test_results_repeat(kind, shape):
+    c = Case(95, **shape, softcap=9.0)
+    first = c.run()
+    assert all(torch.equal(c.run(), first) for _ in range(5))
