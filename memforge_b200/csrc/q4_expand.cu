@@ -3,13 +3,16 @@
 // them by TMA (attn_prefill_body.cuh, EXP).
 //
 // The converting form of that kernel redoes the conversion for every 128-row tile, and its
-// converters' 3000 instructions a key tile share the SM with the softmax: 913 us for four ragged
-// chunks of 300..2048 rows (32/8 heads), 665 us in this form, 649 us from a 16-bit pool.  It costs
-// 512 bytes of writes per token and kv head, once, and is used from six row tiles of a kv head
-// on, while the expanded copy (bounded by the tables' width) stays below SCRATCH_MAX.  Against
-// converting, 16 sequences of 2000 / 8000 keys, 8 kv heads: four tiles 114 : 116 / 393 : 331 us,
-// six 149 : 167 / 510 : 487, eight 176 : 199 / 605 : 607, sixteen 293 : 370 / 1038 : 1185; four
-// sequences, six tiles: 50 : 59 / 150 : 159.
+// converters' 3000 instructions a key tile share the SM with the softmax.  Expanding costs 512
+// bytes of writes per token and kv head, once.  It is used from five row tiles of a kv head on,
+// while the expanded copy (bounded by the tables' width) stays below SCRATCH_MAX.  Expanded :
+// converting in us (device, 32/8 heads, every run of the given tiles at the end of its keys):
+//
+//   tiles                          3          4          5          6          8           16
+//   4 sequences of 2000 keys   41 :  43   42 :  43   60 :  76   61 :  78   62 :  77    99 :  141
+//   4 of 8000                 121 : 115  122 : 116  189 : 218  189 : 228  189 : 226   325 :  438
+//   16 of 2000                117 : 114  134 : 149  154 : 179  174 : 216  191 : 248   322 :  462
+//   16 of 8000                381 : 338  453 : 454  525 : 590  599 : 670  670 : 817  1160 : 1498
 
 #include <algorithm>
 
@@ -21,7 +24,7 @@ namespace mf {
 namespace pf {
 
 constexpr size_t SCRATCH_MAX = size_t(1) << 30;
-constexpr int MIN_ROWS = 6 * BM;
+constexpr int MIN_TILES = 5;  // row tiles of a kv head
 
 template <typename T, bool MOD>
 __global__ void __launch_bounds__(THREADS, 1) q4_expanded_kernel(
@@ -199,8 +202,9 @@ static int launch_expanded(const Params& P, const CUtensorMap& mq, const CUtenso
 bool q4_expand_plan(const AttnParams& a, int width, int vec, mf_dtype dtype, Q4Scratch& sc) {
   const int G = a.hq / a.hkv;
   if (!vec || (int64_t)a.total_q * a.hq > 0x7fffffffLL - 16) return false;
-  if (!q4_prefill_serves(a, dtype) || G > 16 || (int64_t)a.max_q_len * G < pf::MIN_ROWS)
-    return false;
+  if (!q4_prefill_serves(a, dtype) || G > 16) return false;
+  const int ppt = pf::positions_per_tile(G);
+  if ((a.max_q_len + ppt - 1) / ppt < pf::MIN_TILES) return false;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const double rows = (double)a.num_seqs * width * q4::BLOCK * a.hkv;
   if (rows * pf::D * 4 > (double)pf::SCRATCH_MAX || a.num_seqs > 65535) return false;

@@ -41,7 +41,7 @@ def form(num_seqs, q_per_seq, hq, hkv, width, rows):
     return "expanded" if need > least else "converting" if need == 0 else "mma.sync"
 
 
-CONVERTING = dict(hq=16, hkv=4, kv=[200, 527, 640], ql=150)   # 60 row tiles of 16 a head, 5 of 128
+CONVERTING = dict(hq=16, hkv=4, kv=[200, 527, 640], ql=125)   # 32 row tiles of 16 a head, 4 of 128
 EXPANDED = dict(hq=16, hkv=4, kv=[200, 527, 640], ql=200)     # 7 of 128
 
 
@@ -241,17 +241,17 @@ def test_windows_and_prefixes_around_pages_and_tiles(kind, shape, window):
 
 @pytest.mark.parametrize("kind,shape", FORMS)
 def test_non_causal_and_contexts_shorter_than_their_rows(kind, shape):
-    shape = dict(shape, kv=[0, 130, 400])
+    shape = dict(shape, kv=[0, 100, 400])
     c = Case(88, **shape)
     assert c.form() == kind
     got = c.check()
     ql = shape["ql"]
-    assert not got[:ql].any() and not got[ql:2 * ql - 130].any() and got[2 * ql - 130].any()
+    assert not got[:ql].any() and not got[ql:2 * ql - 100].any() and got[2 * ql - 100].any()
     Case(89, **shape, causal=False).check()
 
 
 @pytest.mark.parametrize("kind,hq,hkv,ql", [
-    ("converting", 4, 4, 700), ("converting", 28, 4, 100), ("converting", 40, 5, 80),
+    ("converting", 8, 8, 400), ("converting", 35, 5, 70), ("converting", 40, 5, 60),
     ("converting", 96, 3, 60), ("converting", 128, 4, 23), ("converting", 84, 4, 40),
     ("expanded", 4, 4, 800), ("expanded", 28, 4, 120), ("expanded", 80, 5, 56),
     ("expanded", 27, 3, 300)])
