@@ -455,7 +455,12 @@ MF_API int mf_q4_gather_kv(const void* pool, int64_t pool_stride_block, int64_t 
  * visible key (kv_len 0, or kv_len < q_len) is written as zeros, without an error.
  * A negative kv_len or a run longer than max_q_len sets MF_ERR_LENGTH, a table too short
  * for kv_len MF_ERR_TABLE (the keys behind it are left out), a block id outside the
- * pool MF_ERR_BLOCK_ID (block 0 is read in its place).
+ * pool MF_ERR_BLOCK_ID (block 0 is read in its place).  A NaN row (K or V) makes NaN of the
+ * rows that see it and of no others.  Entries of row_map behind the last sequence's rows
+ * are not read.
+ *
+ * Values are n * scale + base; long bf16 runs (head_dim 128) round that to fp16 once, and take
+ * what passes 65504 (by 120 at most, in a row that reaches it) as 65504.
  *
  * The workspace (16-byte aligned) is scratch: it needs no initial value and nothing
  * in it outlives the call, but calls that may overlap must not share one.

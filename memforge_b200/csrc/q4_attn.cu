@@ -1116,6 +1116,7 @@ int to_q4_params(const mf_q4_attention_args* a, int32_t* err, q4a::Params& P) {
 // expand: may long runs read an expanded copy of the cache (else they convert as they go)
 Plan make_plan(q4a::Params& P, mf_dtype dt, int sms, bool expand = true) {
   Plan pl{};
+  P.rows_cap = 0;
   int64_t rows = (int64_t)P.a.max_q_len * P.G;
   pl.chunks = P.width > 0 && chunks_win(rows, (int64_t)P.a.num_seqs * P.a.hkv, sms) && q4_prefill_serves(P.a, dt);
   pl.expand = expand && pl.chunks && q4_expand_plan(P.a, P.width, P.vec, dt, pl.scratch);
