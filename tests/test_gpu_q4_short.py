@@ -11,6 +11,7 @@ import torch
 
 from tests import q4_bounds as B
 from tests import q4_reference as R
+from tests.gpu_util import TORCH_DT
 from tests.test_gpu_q4 import as_dtype, rng, tables_for
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +86,31 @@ def test_modified_scores(dtype, mods):
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_long_runs_of_the_types_that_stay(dtype):
     check(303, dtype, 8, 2, 128, [420, 260], 150)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("hq,hkv,d,ql,tokens", [(16, 8, 128, 1, 131072), (16, 8, 128, 5, 60000),
+                                                (8, 8, 64, 1, 131072), (8, 8, 256, 1, 40000)])
+def test_sums_over_long_contexts(dtype, hq, hkv, d, ql, tokens):
+    """Flat weights (q = 0) over many keys: the output is the values' mean, far smaller than they
+    are, so a sum that loses a little of itself with each key would show.  Enough sequences (of
+    the same pages) that a thread block takes whole contexts."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    seqs, blocks = 72, tokens // 16
+    pool = torch.zeros((blocks, hkv, R.record_bytes(d)), dtype=torch.uint8, device="cuda")
+    rows = torch.randn((2, tokens, hkv, d), generator=g, device="cuda")
+    index = torch.arange(tokens, device="cuda")
+    K.q4_reshape_and_cache(rows[0], rows[1], pool, index)
+    values = K.q4_gather_kv(pool, index, torch.float32)[1][0].double()     # (H, tokens, d)
+    q = torch.zeros((seqs * ql, hq, d), device="cuda").to(TORCH_DT[dtype])
+    out = torch.full_like(q, 7.0)
+    tables = torch.arange(blocks, dtype=torch.int32, device="cuda").expand(seqs, -1).contiguous()
+    kv = torch.full((seqs,), tokens, dtype=torch.int32, device="cuda")
+    K.q4_paged_attention(q, out, pool, tables, kv, q_per_seq=ql, scale=1 / math.sqrt(d))
+    K.check_device_errors()
+    sums = values.sum(1) - torch.stack([values[:, tokens - ql + 1 + i:].sum(1) for i in range(ql)])
+    count = tokens - ql + 1 + torch.arange(ql, device="cuda").view(-1, 1, 1)
+    want = (sums / count).repeat_interleave(hq // hkv, 1)                   # (ql, hq, d)
+    got = out.view(seqs, ql, hq, d).double()
+    off = (got - want).square().mean().sqrt()
+    assert off <= B.RMS[dtype] * want.square().mean().sqrt()
