@@ -21,7 +21,7 @@ from . import paged_gather
 # What the cache, the attention function and the graphed decoder ask of a pool.  A pool that
 # holds rows in a form of its own brings attend, write_rows, device and spec (PagedKVPool,
 # Q4KVPool); of any other object, MemForge's own pool among them, key_pool, value_pool and
-# block_size are enough.
+# block_size are enough (the graphed decoder reads spec.num_layers too, the cache its own methods).
 
 def pool_device(pool) -> torch.device:
     return pool.key_pool.device if hasattr(pool, "key_pool") else pool.device
