@@ -569,10 +569,10 @@ MF_DEVINL void q4_stage(const Params& P, const int* prefix, const uint16_t* orde
             asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
                          : "=r"(pr[u][0]), "=r"(pr[u][1])
                          : "r"(rec + par_off));
-          else
-            asm volatile("ld.shared.u32 %0, [%2];\n\tld.shared.u32 %1, [%2 + 64];"  // K's, V's
-                         : "=r"(pr[u][0]), "=r"(pr[u][1])
-                         : "r"(rec + par_off));
+          else {  // K's parameters and V's
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pr[u][0]) : "r"(rec + par_off));
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pr[u][1]) : "r"(rec + par_off + 64));
+          }
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
